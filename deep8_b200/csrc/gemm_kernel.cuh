@@ -1256,6 +1256,9 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                         cur = old;
                     }
                     s_last = (static_cast<int>(drawn) == p.splits);
+                    // all tickets of this launch are drawn: the word goes back to none, so that a launch captured into a graph, whose
+                    // epoch is the same at every replay, finds it as the first time
+                    if (s_last) *reinterpret_cast<volatile unsigned*>(word) = fresh;
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (s_last) {
