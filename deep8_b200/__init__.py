@@ -3,6 +3,6 @@ forward and gradients) behind a C ABI (include/d8k.h).  This Python package is a
 used by the tests and the benchmark; device memory comes from torch tensors."""
 from . import _lib
 from ._lib import F16, F32, D8kError
-from .ops import Context
+from .ops import ACTIVATIONS, Context, Dropout
 
-__all__ = ["Context", "F16", "F32", "D8kError"]
+__all__ = ["ACTIVATIONS", "Context", "Dropout", "F16", "F32", "D8kError"]

@@ -14,6 +14,15 @@ F16, F32 = 0, 1
 
 _vp, _i, _ll, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t
 
+
+
+class DropoutSpec(ctypes.Structure):
+    """d8k_dropout"""
+    _fields_ = [("p", ctypes.c_double), ("seed", ctypes.c_ulonglong), ("offset", ctypes.c_ulonglong), ("device_offset", _vp)]
+
+
+_drop = ctypes.POINTER(DropoutSpec)
+
 # name -> (restype, argtypes); mirrors include/d8k.h one to one
 SIGNATURES = {
     "d8k_ctx_create": (_i, [_i, _sz, ctypes.POINTER(_vp)]),
@@ -71,6 +80,15 @@ SIGNATURES = {
     "d8k_sum_shards_gather": (_i, [_vp, _i, _vp, ctypes.POINTER(_vp), _i, _sz, _vp, ctypes.c_float, ctypes.c_float, ctypes.POINTER(_vp), _i]),
     "d8k_axpby": (_i, [_vp, _i, _vp, ctypes.c_float, _vp, ctypes.c_float, _sz]),
     "d8k_sum_shards_sgd": (_i, [_vp, _i, _vp, ctypes.POINTER(_vp), _i, _sz, _vp, ctypes.c_float, ctypes.c_float]),
+    "d8k_gated_forward": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _drop]),
+    "d8k_gated_grad_pre": (_i, [_vp, _i, _i, _vp, _vp, _vp, _sz, _drop]),
+    "d8k_gated_grad_x_into": (_i, [_vp, _i, _vp, _i, _i, _i, _vp, _i, _vp, _i]),
+    "d8k_gated_grad_w_into": (_i, [_vp, _i, _vp, _i, _i, _i, _vp, _i, _vp, _i]),
+    "d8k_gated_backward": (_i, [_vp, _i, _i, _vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _drop]),
+    "d8k_dropout_forward": (_i, [_vp, _i, _vp, _vp, _vp, _sz, _drop]),
+    "d8k_dropout_backward": (_i, [_vp, _i, _vp, _vp, _sz, _i, _drop]),
+    "d8k_rms_norm_forward": (_i, [_vp, _i, _vp, _vp, ctypes.c_float, _vp, _vp, _sz, _i]),
+    "d8k_rms_norm_backward": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _i]),
 }
 
 IPC_HANDLE_BYTES = 64

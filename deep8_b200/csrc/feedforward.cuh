@@ -1,0 +1,84 @@
+// Device arithmetic of the gated feed-forward block's operators, shared by their own kernels and by the contraction kernels'
+// epilogues: the activations with their derivatives, and the counter-based generator behind dropout.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace d8k {
+
+// values of the activation argument (D8K_ACT_* in d8k.h)
+enum : int { kActSilu = 0, kActGelu = 1, kActGeluTanh = 2, kActRelu = 3, kActSigmoid = 4, kActCount = 5 };
+
+// 1 / (1 + exp(-a)).  FAST (results that are rounded to fp16, whose step is 2^-11): the hardware exponential and a division
+// without the last rounding, a few 2^-22 together; otherwise the library's exponential and an IEEE division.
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_of(float a) {
+    if (a < -80.0f) return 0.0f;  // under 2^-115; exp(80) keeps both divisions in their full range
+    if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(-a));
+    else return 1.0f / (1.0f + expf(-a));
+}
+
+// value = act(a); slope = act'(a) when wanted.  gelu goes through erfc, gelu_tanh through a sigmoid ((1 + tanh z) / 2 = sigmoid(2 z)):
+// both forms keep the relative accuracy of the negative tail, where 1 + erf and 1 + tanh cancel.  Arguments beyond +-80 take the
+// limits' values (an fp16 projection may have overflowed to an infinity, and infinity times a vanished factor would be a NaN).
+template <bool FAST, bool SLOPE>
+__device__ __forceinline__ void activation(int act, float a, float& value, float& slope) {
+    const float lo = a < -80.0f ? -80.0f : a;
+    const float b = lo > 80.0f ? 80.0f : lo;
+    if (act == kActSilu || act == kActSigmoid) {
+        const float s = sigmoid_of<FAST>(a);
+        const float ds = s * (1.0f - s);
+        value = act == kActSilu ? lo * s : s;
+        if (SLOPE) slope = act == kActSilu ? fmaf(b, ds, s) : ds;
+    } else if (act == kActGeluTanh) {
+        const float c2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
+        const float b2 = b * b;
+        const float s = sigmoid_of<FAST>(c2 * b * fmaf(0.044715f, b2, 1.0f));
+        value = lo * s;
+        if (SLOPE) slope = fmaf(b * s * (1.0f - s), c2 * fmaf(0.134145f, b2, 1.0f), s);
+    } else if (act == kActGelu) {
+        const float cdf = 0.5f * erfcf(-0.7071067811865476f * b);
+        value = lo * cdf;
+        if (SLOPE) slope = fmaf(b * 0.3989422804014327f, FAST ? __expf(-0.5f * b * b) : expf(-0.5f * b * b), cdf);
+    } else {  // relu: a NaN gives 0, as in the framework's ReLU
+        value = a > 0.0f ? a : 0.0f;
+        if (SLOPE) slope = a > 0.0f ? 1.0f : 0.0f;
+    }
+}
+
+// Philox4x32-10 (Salmon, Moraes, Dror, Shaw: Parallel random numbers: as easy as 1, 2, 3, SC 2011): four 32-bit words from a
+// 128-bit counter under a 64-bit key.  The words of one counter are dropout's decisions for four consecutive elements, so a
+// mask is a function of (seed, offset, element) and is computed again wherever it is needed instead of being stored.
+__device__ __forceinline__ uint4 philox4x32(unsigned long long group, unsigned long long offset, unsigned long long seed) {
+    uint32_t c0 = static_cast<uint32_t>(group), c1 = static_cast<uint32_t>(group >> 32);
+    uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
+    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const unsigned long long a = static_cast<unsigned long long>(c0) * 0xD2511F53u, b = static_cast<unsigned long long>(c2) * 0xCD9E8D57u;
+        c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+        c1 = static_cast<uint32_t>(b);
+        c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+        c3 = static_cast<uint32_t>(a);
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return make_uint4(c0, c1, c2, c3);
+}
+
+// What a kernel needs to decide element i: it stays when word i % 4 of counter (i / 4, offset) is at least `threshold`
+// (p * 2^32), and is then multiplied by `scale` (1 / (1 - p)).  `counter` (device memory, may be null) is added to `offset` when the kernel
+// runs, so that a captured graph draws new masks at every replay.
+struct DropSpec {
+    unsigned long long seed, offset;
+    const unsigned long long* counter;
+    uint32_t threshold;
+    int some;  // 0: p == 1, nothing stays
+    float scale;
+};
+__device__ __forceinline__ unsigned long long drop_offset(const DropSpec& d) { return d.offset + (d.counter ? *d.counter : 0ull); }
+__device__ __forceinline__ bool drop_keeps(const DropSpec& d, uint32_t word) { return d.some && word >= d.threshold; }
+
+}  // namespace d8k

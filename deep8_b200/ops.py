@@ -48,12 +48,36 @@ def _same(*ts):
     return _dtype_code(d0)
 
 
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3, "sigmoid": 4}  # D8K_ACT_*
+
+
+class Dropout:
+    """A dropout mask that is computed wherever it is needed and never stored (d8k_dropout): element i stays when word i % 4 of
+    Philox4x32-10 at the counter (i / 4, offset + counter) under `seed` is at least p * 2^32, and is then multiplied by 1 / (1 - p).
+    The backward pass gives the same object (or one with the same values); calls whose masks are to differ give different
+    offsets.  counter: optional int64 tensor of one element on the GPU, read when the kernel runs, so that a captured graph
+    which advances it draws a new mask at every replay."""
+
+    __slots__ = ("p", "seed", "offset", "counter", "arg")
+
+    def __init__(self, p, seed, offset=0, counter=None):
+        if not 0.0 <= p <= 1.0:
+            raise ValueError("dropout: p must be between 0 and 1")
+        if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+            raise ValueError("dropout: seed and offset are unsigned 64-bit integers")
+        if counter is not None and (counter.dtype != torch.int64 or counter.numel() != 1):
+            raise ValueError("dropout: the counter is an int64 tensor of one element")
+        self.p, self.seed, self.offset, self.counter = float(p), int(seed), int(offset), counter
+        self.arg = ctypes.byref(_lib.DropoutSpec(self.p, self.seed, self.offset, counter.data_ptr() if counter is not None else None))
+
+
 class Context:
     """One d8k context: a device, a stream and the split-K scratch memory.  Not for concurrent use."""
 
     def __init__(self, device=0, scratch_bytes=0):
         self.lib = _lib.load()
         self.device = device
+        self.stream = None  # torch.cuda.Stream given to use_stream
         h = ctypes.c_void_p()
         check(self.lib.d8k_ctx_create(device, scratch_bytes, ctypes.byref(h)))
         self.h = h
@@ -73,6 +97,7 @@ class Context:
     def use_stream(self, stream):
         """Enqueue on a torch.cuda.Stream (or None for the legacy default stream)."""
         check(self.lib.d8k_ctx_set_stream(self.h, ctypes.c_void_p(stream.cuda_stream if stream is not None else 0)))
+        self.stream = stream
 
     def status(self):
         s = ctypes.c_int(0)
@@ -317,6 +342,144 @@ class Context:
     def zero(self, t):
         check(self.lib.d8k_zero(self.h, _p(t), t.numel() * t.element_size()))
         return t
+
+    # ------------------------------------------------------------------------------------------------ gated feed-forward block
+    def _on_device(self, *ts):
+        """_same, and on this context's GPU."""
+        dt = _same(*ts)
+        if not ts[0].is_cuda or ts[0].device.index != self.device:
+            raise ValueError("the device type must be same")
+        return dt
+
+    def _drop_arg(self, dropout):
+        if dropout is None:
+            return None
+        if dropout.counter is not None and (not dropout.counter.is_cuda or dropout.counter.device.index != self.device):
+            raise ValueError("the device type must be same")
+        return dropout.arg
+
+    @staticmethod
+    def _activation(name):
+        try:
+            return ACTIVATIONS[name]
+        except (KeyError, TypeError):
+            raise ValueError("no such activation: %r" % (name,)) from None
+
+    @staticmethod
+    def _gated_dims(x, w):
+        if x.dim() != 3 or w.dim() != 3:
+            raise ValueError("the shape is error")
+        xb, xr, xc = x.shape
+        two, wr, yc = w.shape
+        if two != 2 or wr != xc or xc < 1 or yc < 1:
+            raise ValueError("the shape is error")
+        return xb, xr, xc, yc
+
+    def gated_forward(self, x, w, activation="silu", out=None, pre=None, dropout=None):
+        """h = act(x w[0]) * (x w[1]) in one launch, then `dropout` (a Dropout) on h.  x [xb, xr, xc], w [2, xc, yc] (the gate and the up
+        projection), h [xb, xr, yc].  pre [2, xb * xr, yc] receives both projections, which the backward pass reads; None when
+        there is none to come."""
+        dt = self._on_device(x, w) if pre is None else self._on_device(x, w, pre)
+        xb, xr, xc, yc = self._gated_dims(x, w)
+        act = self._activation(activation)
+        if pre is not None and tuple(pre.shape) != (2, xb * xr, yc):
+            raise ValueError("the shape is error")
+        drop = self._drop_arg(dropout)
+        h = _out(out, (xb, xr, yc), x)
+        check(self.lib.d8k_gated_forward(self.h, dt, act, _p(x), xb, xr, xc, _p(w), yc, _p(pre), _p(h), drop))
+        return h
+
+    def gated_grad_pre(self, pre, dz, activation="silu", dpre=None, dropout=None):
+        """Gradient of pre [2, rows, yc] from dz, the gradient of h (rows * yc elements); dpre may be pre."""
+        dt = self._on_device(pre, dz)
+        if pre.dim() != 3 or pre.shape[0] != 2 or 2 * dz.numel() != pre.numel():
+            raise ValueError("the shape is error")
+        act, drop = self._activation(activation), self._drop_arg(dropout)
+        dpre = _out(dpre, tuple(pre.shape), pre)
+        check(self.lib.d8k_gated_grad_pre(self.h, dt, act, _p(pre), _p(dz), _p(dpre), dz.numel(), drop))
+        return dpre
+
+    def gated_backward(self, x, w, pre, dz, dx, dw, activation="silu", dpre=None, accumulate=True, dropout=None):
+        """dx (+)= and dw (+)= the gradients of gated_forward's x and w for h's gradient dz [xb, xr, yc]; dx or dw may be None.  pre is what
+        gated_forward stored, dropout the same mask; dpre [2, xb * xr, yc] is workspace (may be pre, which is then overwritten)."""
+        dt = self._on_device(x, w, pre, dz)
+        xb, xr, xc, yc = self._gated_dims(x, w)
+        if tuple(pre.shape) != (2, xb * xr, yc) or tuple(dz.shape) != (xb, xr, yc):
+            raise ValueError("the shape is error")
+        for grad, like in ((dx, x), (dw, w)):
+            if grad is not None:
+                _same(like, grad)
+                if grad.shape != like.shape:
+                    raise ValueError("the shape is error")
+        act, drop = self._activation(activation), self._drop_arg(dropout)
+        if dpre is None:
+            dpre = self._workspace(pre)
+        else:
+            dpre = _out(dpre, tuple(pre.shape), pre)
+        check(self.lib.d8k_gated_backward(self.h, dt, act, _p(x), xb, xr, xc, _p(w), yc, _p(pre), _p(dz), _p(dpre), _p(dx), _p(dw),
+                                          int(accumulate), drop))
+        return dx, dw
+
+    def _workspace(self, like):
+        """Temporary memory for one call, from the pool of the stream that this context enqueues on: torch may hand it out again
+        as soon as the call returns, and whatever gets it then is enqueued behind the call's kernels."""
+        with torch.cuda.stream(self.stream if self.stream is not None else torch.cuda.default_stream(self.device)):
+            return torch.empty_like(like)
+
+    def dropout_forward(self, x, dropout, residual=None, out=None):
+        """(residual +) x with elements dropped; out may be x or residual."""
+        dt = self._on_device(x) if residual is None else self._on_device(x, residual)
+        if residual is not None and residual.shape != x.shape:
+            raise ValueError("the shape is error")
+        drop = self._drop_arg(dropout)
+        y = _out(out, tuple(x.shape), x)
+        check(self.lib.d8k_dropout_forward(self.h, dt, _p(x), _p(residual), _p(y), x.numel(), drop))
+        return y
+
+    def dropout_backward(self, dx, dy, dropout, accumulate=True):
+        """dx (+)= dy through the same mask; without accumulation dx may be dy.  (The residual's gradient is dy.)"""
+        dt = self._on_device(dx, dy)
+        if dx.shape != dy.shape:
+            raise ValueError("the shape is error")
+        check(self.lib.d8k_dropout_backward(self.h, dt, _p(dx), _p(dy), dy.numel(), int(accumulate), self._drop_arg(dropout)))
+        return dx
+
+    @staticmethod
+    def _check_rstd(rstd, rows, like):
+        if rstd.dtype != torch.float32 or not rstd.is_contiguous() or rstd.device != like.device:
+            raise ValueError("rstd is a contiguous float32 tensor on the same device")
+        if rstd.numel() != rows:
+            raise ValueError("the shape is error")
+
+    def rms_norm_forward(self, x, weight, eps=1e-6, out=None, rstd=None):
+        """y = x * rstd * weight, rstd = 1 / sqrt(mean(x^2) + eps) over the last dimension.  rstd: optional float32 tensor with one element per
+        row that receives the factors the backward pass reads; out may be x."""
+        dt = self._on_device(x, weight)
+        if x.dim() < 1 or x.shape[-1] < 1 or weight.numel() != x.shape[-1]:
+            raise ValueError("the shape is error")
+        cols = x.shape[-1]
+        rows = x.numel() // cols
+        if rstd is not None:
+            self._check_rstd(rstd, rows, x)
+        y = _out(out, tuple(x.shape), x)
+        check(self.lib.d8k_rms_norm_forward(self.h, dt, _p(x), _p(weight), float(eps), _p(y), _p(rstd), rows, cols))
+        return y
+
+    def rms_norm_backward(self, x, weight, rstd, dx, dweight, dy, accumulate=True):
+        """dx (+)= and dweight (+)= the gradients of rms_norm_forward for dy; dx or dweight may be None."""
+        dt = self._on_device(x, weight, dy)
+        if x.dim() < 1 or x.shape[-1] < 1 or weight.numel() != x.shape[-1] or dy.shape != x.shape:
+            raise ValueError("the shape is error")
+        cols = x.shape[-1]
+        rows = x.numel() // cols
+        self._check_rstd(rstd, rows, x)
+        for grad, like in ((dx, x), (dweight, weight)):
+            if grad is not None:
+                _same(like, grad)
+                if grad.shape != like.shape:
+                    raise ValueError("the shape is error")
+        check(self.lib.d8k_rms_norm_backward(self.h, dt, _p(x), _p(weight), _p(rstd), _p(dx), _p(dweight), _p(dy), rows, cols, int(accumulate)))
+        return dx, dweight
 
     # ------------------------------------------------------------------------------------------------ exchange between GPUs
     # Raw device addresses (ints): the memory belongs to the library (d8k_peer_alloc) or to a peer process.

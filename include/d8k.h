@@ -267,6 +267,59 @@ D8K_API int d8k_sum_shards_adam(d8k_ctx* ctx, int dtype, void* grad_out, const v
                                 void* v, float beta1, float beta2, float epsilon, float learning_rate, float weight_decay, long long steps,
                                 void* const* copies, int ncopies);
 
+/* ---- A gated feed-forward block: y = residual + dropout((act(n w0) * (n w1)) w2) with n = rms_norm(x).  No counterpart in the
+ * reference, whose feed-forward layer is MatrixMultiply - ReLu - MatrixMultiply; w2's product is d8k_matmul_forward.
+ * These entry points run on the context's device whatever device is current, refuse outputs that overlap inputs unless they say
+ * otherwise, and may be captured into a graph (one graph of a context replays at a time: they share its scratch memory). */
+#define D8K_ACT_SILU 0      /* a / (1 + exp(-a)) */
+#define D8K_ACT_GELU 1      /* a * (1 + erf(a / sqrt(2))) / 2 */
+#define D8K_ACT_GELU_TANH 2 /* a * (1 + tanh(sqrt(2 / pi) * (a + 0.044715 a^3))) / 2 */
+#define D8K_ACT_RELU 3      /* max(a, 0) */
+#define D8K_ACT_SIGMOID 4   /* 1 / (1 + exp(-a)) */
+
+/* A dropout mask, which is never stored: element i (flat index in its tensor) stays when word i % 4 of Philox4x32-10 at the counter
+ * (i / 4, offset + *device_offset) under key = seed is at least p * 2^32, and is then multiplied by 1 / (1 - p); dropped elements
+ * are 0 whatever they held.  0 <= p <= 1.  A mask is used again (in a backward pass) by giving the same seed and offset; calls
+ * that are to differ give different ones.  device_offset (a device pointer to one 64-bit word, or NULL for 0) is read when the
+ * kernel runs: a captured graph that advances the word draws a new mask at every replay. */
+typedef struct d8k_dropout {
+    double p;
+    unsigned long long seed, offset;
+    const unsigned long long* device_offset;
+} d8k_dropout;
+
+/* pre[b] = x * w[b], b = 0, 1, and h = act(pre[0]) * pre[1], then dropout on h when drop is not NULL, in one launch.
+ * x is xb matrices xr x xc whose rows are taken together, w two matrices xc x yc (gate and up projection, one tensor), h has xb * xr rows of
+ * yc; pre, 2 x (xb * xr) x yc, is what the backward pass needs, or NULL.  h comes from the fp32 accumulators with one rounding.  xb * xr may be 0. */
+D8K_API int d8k_gated_forward(d8k_ctx* ctx, int dtype, int activation, const void* x, int xb, int xr, int xc, const void* w, int yc, void* pre,
+                              void* h, const d8k_dropout* drop);
+/* The gradient of pre from h's: with d = dz through the dropout, dpre[0] = d * pre[1] * act'(pre[0]) and dpre[1] = d * act(pre[0]), n = rows * yc
+ * elements each (pre and dpre hold 2 n).  dpre may be pre. */
+D8K_API int d8k_gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, const void* dz, void* dpre, size_t n,
+                               const d8k_dropout* drop);
+/* dx (+)= dpre[0] * w[0]^T + dpre[1] * w[1]^T, one launch; accumulate == 0 overwrites, as in d8k_matmul_grad_x_into. */
+D8K_API int d8k_gated_grad_x_into(d8k_ctx* ctx, int dtype, void* dx, int xb, int xr, int xc, const void* w, int yc, const void* dpre,
+                                  int accumulate);
+/* dw[b] (+)= x^T * dpre[b], one launch for both. */
+D8K_API int d8k_gated_grad_w_into(d8k_ctx* ctx, int dtype, const void* x, int xb, int xr, int xc, void* dw, int yc, const void* dpre,
+                                  int accumulate);
+/* The three above: dpre (2 x rows x yc, workspace; may be pre) from pre and dz, then dx and dw; dx or dw may be NULL. */
+D8K_API int d8k_gated_backward(d8k_ctx* ctx, int dtype, int activation, const void* x, int xb, int xr, int xc, const void* w, int yc,
+                               const void* pre, const void* dz, void* dpre, void* dx, void* dw, int accumulate, const d8k_dropout* drop);
+
+/* y = (residual +) dropout(x) over n elements; residual may be NULL, y may be x or residual. */
+D8K_API int d8k_dropout_forward(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* y, size_t n, const d8k_dropout* drop);
+/* dx (+)= dropout(dy) with the forward pass's mask; accumulate == 0 overwrites, and then dx may be dy.  (The residual's gradient is dy.) */
+D8K_API int d8k_dropout_backward(d8k_ctx* ctx, int dtype, void* dx, const void* dy, size_t n, int accumulate, const d8k_dropout* drop);
+
+/* rstd[r] = 1 / sqrt(mean of x[r][.]^2 + eps), y[r][c] = x[r][c] * rstd[r] * weight[c]; sums in fp32.  rstd: rows floats whatever the
+ * dtype, what the backward pass needs, or NULL.  y may be x. */
+D8K_API int d8k_rms_norm_forward(d8k_ctx* ctx, int dtype, const void* x, const void* weight, float eps, void* y, float* rstd, size_t rows, int cols);
+/* With u = dy * weight and n = x * rstd: dx (+)= rstd * (u - n * mean(u * n)) and dweight[c] (+)= sum over r of dy[r][c] * n[r][c], added in a fixed
+ * order (same bits every run); dx or dweight may be NULL.  Uses the context's scratch memory. */
+D8K_API int d8k_rms_norm_backward(d8k_ctx* ctx, int dtype, const void* x, const void* weight, const float* rstd, void* dx, void* dweight,
+                                  const void* dy, size_t rows, int cols, int accumulate);
+
 #ifdef __cplusplus
 }
 #endif
