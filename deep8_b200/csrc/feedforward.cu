@@ -25,70 +25,6 @@ namespace {
     } while (0)
 
 // ------------------------------------------------------------------------------------------------ gated projections
-// Plain tiles: 64 x 64 outputs of both projections per CTA, 16 steps of the contraction at a time in shared memory, 4 x 4 outputs of each
-// projection per thread, fp32 multiply-adds.
-template <typename T>
-__global__ void __launch_bounds__(256) gated_forward_kernel(const T* __restrict__ x, const T* __restrict__ w, T* __restrict__ pre, T* __restrict__ h,
-                                                            int rows, int cols, int width, int act, DropSpec drop, int dropping) {
-    constexpr bool FAST = sizeof(T) == 2;
-    __shared__ float xs[16][64 + 1], gs[16][64], us[16][64];
-    const long long r0 = static_cast<long long>(blockIdx.x) * 64;
-    const int c0 = blockIdx.y * 64;
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    float g[4][4] = {}, u[4][4] = {};
-    for (int k0 = 0; k0 < cols; k0 += 16) {
-        for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-            const int r = i >> 4, k = i & 15;
-            xs[k][r] = (r0 + r < rows && k0 + k < cols) ? widen(x[(r0 + r) * cols + k0 + k]) : 0.0f;
-            const int kk = i >> 6, c = i & 63;
-            const bool in = k0 + kk < cols && c0 + c < width;
-            const size_t at = static_cast<size_t>(k0 + kk) * width + c0 + c;
-            gs[kk][c] = in ? widen(w[at]) : 0.0f;
-            us[kk][c] = in ? widen(w[static_cast<size_t>(cols) * width + at]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = xs[k][ty * 4 + i];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    g[i][j] = fmaf(a, gs[k][tx + 16 * j], g[i][j]);
-                    u[i][j] = fmaf(a, us[k][tx + 16 * j], u[i][j]);
-                }
-            }
-        }
-        __syncthreads();
-    }
-    const unsigned long long offset = dropping ? drop_offset(drop) : 0;
-    const size_t half = static_cast<size_t>(rows) * width;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const long long r = r0 + ty * 4 + i;
-        if (r >= rows) break;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + tx + 16 * j;
-            if (c >= width) break;
-            const size_t at = static_cast<size_t>(r) * width + c;
-            float value, slope;
-            activation<FAST, false>(act, g[i][j], value, slope);
-            float out = value * u[i][j];
-            if (dropping) {
-                const uint4 words = philox4x32(at >> 2, offset, drop.seed);
-                const uint32_t word = (at & 3) == 0 ? words.x : (at & 3) == 1 ? words.y : (at & 3) == 2 ? words.z : words.w;
-                out = drop_keeps(drop, word) ? out * drop.scale : 0.0f;
-            }
-            if (pre) {
-                pre[at] = narrow<T>(g[i][j]);
-                pre[half + at] = narrow<T>(u[i][j]);
-            }
-            h[at] = narrow<T>(out);
-        }
-    }
-}
-
 // dpre from pre and dz, four consecutive elements (one counter of the generator) per step: 5 accesses per element, bound by HBM.
 // pre and dpre may be the same memory (an element is read and written by one thread), so nothing here is declared __restrict__.
 template <typename T, bool VEC>
@@ -497,18 +433,14 @@ int d8k_gated_forward(d8k_ctx* ctx, int dtype, int activation, const void* x, in
         const size_t es = esize(dtype), xs = es * rows * xc, ws = 2 * es * xc * yc, hs = es * rows * yc;
         if (overlap(h, hs, x, xs) || overlap(h, hs, w, ws) || overlap(pre, 2 * hs, x, xs) || overlap(pre, 2 * hs, w, ws) || overlap(pre, 2 * hs, h, hs))
             return fail(D8K_ERR_ARGUMENT, "gated: an output overlaps an input or the other output");
-        const dim3 grid((rows + 63) / 64, (yc + 63) / 64);
-        if (grid.y > 65535) return fail(D8K_ERR_ARGUMENT, "the shape is too large");
-        auto run = [&](auto zero) {
-            using T = decltype(zero);
-            gated_forward_kernel<T><<<grid, 256, 0, ctx->stream>>>(static_cast<const T*>(x), static_cast<const T*>(w), static_cast<T*>(pre),
-                                                                   static_cast<T*>(h), rows, xc, yc, activation, spec, dropping);
-        };
-        if (dtype == D8K_F32) run(0.0f);
-        else run(__half());
-        D8K_CUDA(cudaGetLastError());
-        count_launch();
-        return 0;
+        GatedProblem g;
+        g.dtype = dtype;
+        g.M = rows; g.N = yc; g.K = xc;
+        g.a = x;
+        g.b = w;
+        g.C = h;
+        g.tail = GatedTail{activation, dropping, pre, 1LL * rows * yc, spec};
+        return run_gated(ctx, g);
     });
 }
 

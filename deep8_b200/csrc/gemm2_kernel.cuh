@@ -28,8 +28,12 @@
 
 namespace d8k {
 
-template <bool A_MN_, bool B_MN_, int STAGES_, int SUB_ = 2>
+template <bool A_MN_, bool B_MN_, int STAGES_, int SUB_ = 2, bool GATED_ = false>
 struct Gemm2Cfg {
+    // GATED (see GemmCfg): CTA 0 of the pair stages 128 columns of the gate projection, CTA 1 the same columns of the up projection; the
+    // accumulator's columns [0, 128) are the gate's, [128, 256) the up projection's, for a tile of 256 x 128 outputs.
+    static constexpr bool GATED = GATED_;
+    static_assert(!GATED_ || B_MN_, "the projections are stored [K, N]");
     static constexpr bool A_MN = A_MN_, B_MN = B_MN_;
     static constexpr int STAGES = STAGES_;
     static constexpr int SUB = SUB_;             // k-blocks of 64 per stage
@@ -223,7 +227,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         for (int w = pair; ok && w < p.total_work; w += num_pairs) {
             PairWork it = decode_pair_work(p, w);
             const int my_m0 = it.m0 + 128 * static_cast<int>(rank);
-            const int my_n0 = it.n0 + Cfg::HALF_N * static_cast<int>(rank);
+            const int my_n0 = Cfg::GATED ? it.n0 / 2 : it.n0 + Cfg::HALF_N * static_cast<int>(rank);
             for (int kk = 0; kk < total_it; ++kk) {
                 const long long tw = p.prof ? clock64() : 0;
                 ok = wait_bar(empty_bar(stage), phase ^ 1, &s_abort, p.status, (kRoleProducer << 8) | 1);
@@ -241,12 +245,13 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     // K-major: {k in block, row, k-block, batch}; MN-major: {m/n in chunk, k, chunk of 64, batch}
                     const int a1 = Cfg::A_MN ? kb0 * 64 : my_m0, a2 = Cfg::A_MN ? my_m0 / 64 : kb0;
                     const int b1 = Cfg::B_MN ? kb0 * 64 : my_n0, b2 = Cfg::B_MN ? my_n0 / 64 : kb0;
+                    const int b3 = Cfg::GATED ? static_cast<int>(rank) : b % p.b_batch_mod;
                     if (hinted) {
                         ptx::tma_load_4d_pair_hint(stage_a(stage), &tmA, bar, 0, a1, a2, b % p.a_batch_mod, pol_a);
-                        ptx::tma_load_4d_pair_hint(stage_b(stage), &tmB, bar, 0, b1, b2, b % p.b_batch_mod, pol_b);
+                        ptx::tma_load_4d_pair_hint(stage_b(stage), &tmB, bar, 0, b1, b2, b3, pol_b);
                     } else {
                         ptx::tma_load_4d_pair(stage_a(stage), &tmA, bar, 0, a1, a2, b % p.a_batch_mod);
-                        ptx::tma_load_4d_pair(stage_b(stage), &tmB, bar, 0, b1, b2, b % p.b_batch_mod);
+                        ptx::tma_load_4d_pair(stage_b(stage), &tmB, bar, 0, b1, b2, b3);
                     }
                 }
                 __syncwarp();
@@ -371,8 +376,62 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             if (p.prof) waited += clock64() - tw;
             ptx::tc_fence_after_sync();
             const uint32_t taddr = tmem_base + acc * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
+            if constexpr (Cfg::GATED) {
+                // 32 columns of both projections at a time; h and, when kept, the projections cross to whole row segments through
+                // the warp's three staging slots
+                const GatedTail& t = p.gated;
+                const bool segments = ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(t.pre)) & 15) == 0 && (p.ldc & 7) == 0 && (t.pre_stride & 7) == 0;
 #pragma unroll 1
-            for (int c = 0; c < 256 / 32; ++c) {
+                for (int c = 0; c < 128 / 32; ++c) {
+                    uint32_t r[32], u[32];
+                    __syncwarp();
+                    ptx::tmem_ld_32x32(taddr + c * 32, r);
+                    ptx::tmem_ld_32x32(taddr + 128 + c * 32, u);
+                    ptx::tmem_ld_wait();
+                    const int col0 = it.n0 / 2 + c * 32;
+                    if (col0 >= p.N) continue;
+                    float gate[32], up[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        gate[i] = __uint_as_float(r[i]);
+                        up[i] = __uint_as_float(u[i]);
+                    }
+                    if (!segments || col0 + 32 > p.N) {
+                        if (row < p.M) store_gated_chunk<OutT>(p, row, col0, gate, up);
+                        continue;
+                    }
+                    const uint32_t s0 = staging, s1 = staging + Cfg::SLOT_BYTES, s2 = staging + 2 * Cfg::SLOT_BYTES;
+                    using V = EpiVec<OutT>;
+                    const uint32_t stays =
+                        t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0) : 0xffffffffu;
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        float h[8];
+                        if (t.pre) {
+                            st_shared_v4(s1 + slot_off(lane, v), V::pack(gate + 8 * v));
+                            st_shared_v4(s2 + slot_off(lane, v), V::pack(up + 8 * v));
+                        }
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) h[i] = gated_value<OutT>(t, gate[8 * v + i], up[8 * v + i], stays >> (8 * v + i) & 1u);
+                        st_shared_v4(s0 + slot_off(lane, v), V::pack(h));
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = 8 * i + lr;
+                        if (warp_row0 + rr < p.M) {
+                            const long long e = static_cast<long long>(warp_row0 + rr) * p.ldc + col0 + lc * 8;
+                            *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(p.C) + e) = ptx::ld_shared_v4(s0 + slot_off(rr, lc));
+                            if (t.pre) {
+                                *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(t.pre) + e) = ptx::ld_shared_v4(s1 + slot_off(rr, lc));
+                                *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(t.pre) + t.pre_stride + e) = ptx::ld_shared_v4(s2 + slot_off(rr, lc));
+                            }
+                        }
+                    }
+                }
+            }
+#pragma unroll 1
+            for (int c = 0; c < (Cfg::GATED ? 0 : 256 / 32); ++c) {
                 uint32_t r[32];
                 __syncwarp();
                 ptx::tmem_ld_32x32(taddr + c * 32, r);

@@ -70,6 +70,16 @@ struct GemmProblem {
     OutMap out = {};  // strided placement of rows / columns in the output tensor (GemmParams::out); FastDivs filled by run_gemm
 };
 
+// act(A B[0]) * (A B[1]) for row-major A [M, K] and B [2, K, N] (GemmCfg::GATED); C [M, N]
+struct GatedProblem {
+    int dtype = 0;
+    int M = 0, N = 0, K = 0;
+    const void* a = nullptr;
+    const void* b = nullptr;
+    void* C = nullptr;
+    GatedTail tail = {};
+};
+
 // error reporting shared by the API layer
 void set_error(const std::string& msg);
 int fail(int code, const std::string& msg);
@@ -91,6 +101,8 @@ struct PreparedGemm {
 
 // capture != nullptr: prepare only (no clearing of tickets, no launch) and hand the result back
 int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture = nullptr);
+// The gated pair of products as one launch; every extent at least 1, every pointer checked by the caller
+int run_gated(Ctx* ctx, const GatedProblem& g);
 // The contractions of one operator (the residue classes of a strided convolution): ONE launch whose work items are all of
 // theirs when the context has a group buffer and every part runs the same one-CTA-per-SM kernel, otherwise one launch each.
 int run_gemm_group(Ctx* ctx, std::vector<GemmProblem>& parts);
@@ -108,6 +120,11 @@ GemmLaunchFn lookup_f32_gather(bool a_mn, bool b_mn, int bn);
 GemmLaunchFn lookup_f32_tma(bool a_mn, bool b_mn, int bn, bool a_in_tmem);
 GemmLaunchFn lookup_f32_dual(bool a_mn, bool b_mn, int mode);  // two CTAs per SM (GemmCfg::DUAL, mode 1 or 2); launch 2 x SMs CTAs
 GemmLaunchFn lookup_f32_halo(bool b_mn);  // K-major virtual A through patches, 64 columns
+// the gated kernels (GemmCfg::GATED), A K-major and B MN-major; the fp32 mode is lookup_f32_dual's
+GemmLaunchFn lookup_f16_gated(int bn);
+GemmLaunchFn lookup_f32_gated(int mode);
+GemmLaunchFn lookup_gated_gather(bool f32);  // loader warps: 128 columns fp16, 64 fp32
+GemmLaunchFn lookup_f16_gated_pair();
 // paired-CTA kernel: the first argument of the launch function is the number of CTA pairs
 GemmLaunchFn lookup_f16_pair(bool a_mn, bool b_mn);
 

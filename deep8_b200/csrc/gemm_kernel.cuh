@@ -36,6 +36,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "feedforward.cuh"
 #include "ptx_sm100.cuh"
 
 namespace d8k {
@@ -128,6 +129,15 @@ struct OutMap {
 
 struct GroupEntry;
 
+// Tail of the gated kernels (GemmCfg::GATED): C = dropout(act(gate) * up), and both projections to `pre` unless it is null (the up
+// projection pre_stride elements behind the gate's).
+struct GatedTail {
+    int act, dropping;
+    void* pre;
+    long long pre_stride;
+    DropSpec drop;
+};
+
 struct GemmParams {
     // Grouped launch (group_count > 1): the work items of several contractions of one operator - the residue classes of a strided
     // convolution - share ONE launch.  `groups` is an array in device memory with each contraction's own parameters and
@@ -174,6 +184,7 @@ struct GemmParams {
     int scatter_rows;
     long long scatter_off[kMaxScatter];
     OutMap out;
+    GatedTail gated;
     GatherSrc a, b;
 };
 
@@ -241,7 +252,8 @@ __device__ __forceinline__ long long scatter_offset(const GemmParams& p, int row
     return p.scatter_off[k < kMaxScatter ? k : kMaxScatter - 1];
 }
 
-template <bool F32_, bool A_MN_, bool B_MN_, int BN_, int STAGES_, bool GATHER_, bool ATMEM_ = false, bool HALO_ = false, int DUAL_ = 0>
+template <bool F32_, bool A_MN_, bool B_MN_, int BN_, int STAGES_, bool GATHER_, bool ATMEM_ = false, bool HALO_ = false, int DUAL_ = 0,
+          bool GATED_ = false>
 struct GemmCfg {
     static constexpr bool F32 = F32_, A_MN = A_MN_, B_MN = B_MN_, GATHER = GATHER_;
     static constexpr int BN = BN_, STAGES = STAGES_;
@@ -322,9 +334,14 @@ struct GemmCfg {
     static constexpr int PRODUCER_B_WARP = BASE_WARPS, MMA2_WARP = BASE_WARPS + 1;  // TWIN only
     static constexpr int THREADS = 32 * (BASE_WARPS + (TWIN ? 2 : 0));
     static_assert(!TWIN || (!GATHER && !HALO_), "the twin roles belong to the TMA kernels");
+    // GATED: B is a pair of stored matrices [2, K, N] (gate and up projection, MN-major).  The first half of a tile's B columns comes from the
+    // gate, the second from the up projection, both from the same BN / 2 columns n0 / 2 onwards, so one accumulator holds both
+    // projections of an output element and the epilogue forms act(gate) * up from it (GatedTail).
+    static constexpr bool GATED = GATED_;
     static constexpr int BAR_BYTES = 256;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + PATCH_SLOTS * PATCH_BYTES + BAR_BYTES + 1024;  // + slack to align the ring to 1024
     static_assert(BN % 16 == 0 && BN >= 16 && BN <= 256, "UMMA N");
+    static_assert(!GATED || (B_MN && BN % (2 * CE) == 0 && !HALO && !GROUPED), "half a gated tile is whole 128-byte chunks of each projection");
     static_assert(BN % CE == 0, "an MN-major B tile is whole 128-byte chunks");
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(DUAL ? SMEM_BYTES <= 112 * 1024 : SMEM_BYTES > 114 * 1024, "one CTA per SM unless DUAL: more would compete for tensor memory");
@@ -770,6 +787,67 @@ __device__ __forceinline__ void store_row_chunk(const GemmParams& p, long long o
     else store_row_chunk_epi<OutT, 4>(p, off, col0, acc);
 }
 
+// Bit k: whether element first + k stays under the dropout, k < 32.  `first` need not be a multiple of the generator's four words.
+__device__ __forceinline__ uint32_t drop_mask32(const DropSpec& d, unsigned long long first) {
+    const unsigned long long offset = drop_offset(d), group = first >> 2;
+    const int skip = static_cast<int>(first & 3);
+    unsigned long long bits = 0;
+#pragma unroll 1
+    for (int g = 0; g < (skip ? 9 : 8); ++g) {
+        const uint4 w = philox4x32(group + g, offset, d.seed);
+        const unsigned long long four = (drop_keeps(d, w.x) ? 1u : 0u) | (drop_keeps(d, w.y) ? 2u : 0u) | (drop_keeps(d, w.z) ? 4u : 0u) | (drop_keeps(d, w.w) ? 8u : 0u);
+        bits |= four << (4 * g);
+    }
+    return static_cast<uint32_t>(bits >> skip);
+}
+
+// h of one element from the accumulated projections; `stays`: the dropout's decision (true without one)
+template <typename OutT>
+__device__ __forceinline__ float gated_value(const GatedTail& t, float gate, float up, bool stays) {
+    float value, slope;
+    activation<sizeof(OutT) == 2, false>(t.act, gate, value, slope);
+    const float h = value * up;
+    return t.dropping ? (stays ? h * t.drop.scale : 0.0f) : h;
+}
+
+// Tail of a gated product for one row and 32 columns [col0, col0 + 32), clipped to N: both projections (when kept) and h, each rounded once.
+template <typename OutT>
+__device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, int col0, const float* gate, const float* up) {
+    using V = EpiVec<OutT>;
+    constexpr int VEC = V::N;
+    const GatedTail& t = p.gated;
+    const long long off = static_cast<long long>(row) * p.ldc + col0;
+    OutT* h = reinterpret_cast<OutT*>(p.C) + off;
+    OutT* pg = t.pre ? reinterpret_cast<OutT*>(t.pre) + off : nullptr;
+    OutT* pu = t.pre ? pg + t.pre_stride : nullptr;
+    const uint32_t stays = t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(off)) : 0xffffffffu;
+    const bool vec_ok = col0 + 32 <= p.N && ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(pg) | reinterpret_cast<uintptr_t>(pu)) & 15) == 0;
+    if (vec_ok) {
+#pragma unroll
+        for (int v = 0; v < 32 / VEC; ++v) {
+            float out[VEC];
+            if (pg) {
+                reinterpret_cast<uint4*>(pg)[v] = V::pack(gate + v * VEC);
+                reinterpret_cast<uint4*>(pu)[v] = V::pack(up + v * VEC);
+            }
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) out[i] = gated_value<OutT>(t, gate[v * VEC + i], up[v * VEC + i], stays >> (v * VEC + i) & 1u);
+            reinterpret_cast<uint4*>(h)[v] = V::pack(out);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {  // fully unrolled: a dynamic index would push the accumulators to local memory
+            if (col0 + i < p.N) {
+                if (pg) {
+                    pg[i] = epi_from_float<OutT>(gate[i]);
+                    pu[i] = epi_from_float<OutT>(up[i]);
+                }
+                h[i] = epi_from_float<OutT>(gated_value<OutT>(t, gate[i], up[i], stays >> i & 1u));
+            }
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ the kernel
 // Producer side of one operand for one stage (one elected lane).  ROWS: tile rows of the operand (kBM or BN); mn0: first
 // row (M or N index) of the tile; k0: first contraction index of the k-block.  Every mode delivers ROWS * 128 bytes.
@@ -995,7 +1073,13 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                     } else {
                         if constexpr (!Cfg::HALO)
                             if (do_a) produce_operand<Cfg, Cfg::A_MN, kBM>(p.a_tma, p.a_chunked, p.a, &tmA, stage_a(stage), bar, k0, it.m0, b % p.a_batch_mod);
-                        if (do_b) produce_operand<Cfg, Cfg::B_MN, BN>(p.b_tma, p.b_chunked, p.b, &tmB, stage_b(stage), bar, k0, it.n0, b % p.b_batch_mod);
+                        if constexpr (Cfg::GATED) {
+                            if (do_b) {
+#pragma unroll
+                                for (int m = 0; m < 2; ++m)
+                                    produce_operand<Cfg, true, BN / 2>(kTmaTiled, p.b_chunked, p.b, &tmB, stage_b(stage) + m * (Cfg::B_BYTES / 2), bar, k0, it.n0 / 2, m);
+                            }
+                        } else if (do_b) produce_operand<Cfg, Cfg::B_MN, BN>(p.b_tma, p.b_chunked, p.b, &tmB, stage_b(stage), bar, k0, it.n0, b % p.b_batch_mod);
                     }
                 }
                 __syncwarp();
@@ -1163,13 +1247,34 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
                 const uint32_t taddr = tmem_base + acc * Cfg::ACC_COLS + (static_cast<uint32_t>(quarter * 32) << 16);
+                if constexpr (Cfg::GATED) {
+                    if (p.splits == 1) {
 #pragma unroll 1
-                for (int c = 0; c < BN / 32; ++c) {
+                        for (int c = 0; c < BN / 64; ++c) {  // 32 columns of the gate and the same 32 of the up projection
+                            uint32_t r[32], s[32];
+                            __syncwarp();
+                            ptx::tmem_ld_32x32(taddr + c * 32, r);
+                            ptx::tmem_ld_32x32(taddr + BN / 2 + c * 32, s);
+                            ptx::tmem_ld_wait();
+                            if (row_ok && it.n0 / 2 + c * 32 < p.N) {
+                                float gate[32], up[32];
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    gate[i] = __uint_as_float(r[i]);
+                                    up[i] = __uint_as_float(s[i]);
+                                }
+                                store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, gate, up);
+                            }
+                        }
+                    }
+                }
+#pragma unroll 1
+                for (int c = 0; c < (Cfg::GATED && p.splits == 1 ? 0 : BN / 32); ++c) {
                     uint32_t r[32];
                     __syncwarp();
                     ptx::tmem_ld_32x32(taddr + c * 32, r);
                     ptx::tmem_ld_wait();
-                    if (p.splits == 1) {
+                    if (!Cfg::GATED && p.splits == 1) {
                         if (row_ok && it.n0 + c * 32 < p.N) {
                             float accv[32];
 #pragma unroll
@@ -1223,10 +1328,18 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                     if (++acc == Cfg::ACC_BUFS) { acc = 0; acc_phase ^= 1; }
                 }
                 if (!ok) break;
+                if constexpr (Cfg::GATED) {
+                    if (p.splits == 1 && row_ok) {
+#pragma unroll
+                        for (int c = 0; c < BN / 64; ++c)
+                            if (it.n0 / 2 + c * 32 < p.N) store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, &accv[c * 32], &accv[BN / 2 + c * 32]);
+                    }
+                }
 #pragma unroll
                 for (int c = 0; c < BN / 32; ++c) {
                     if (p.splits == 1) {
-                        if (row_ok && it.n0 + c * 32 < p.N) store_row_chunk<OutT>(p, crow, it.n0 + c * 32, &accv[c * 32]);
+                        if constexpr (!Cfg::GATED)
+                            if (row_ok && it.n0 + c * 32 < p.N) store_row_chunk<OutT>(p, crow, it.n0 + c * 32, &accv[c * 32]);
                     } else {
 #pragma unroll
                         for (int v = 0; v < 8; ++v)
@@ -1265,8 +1378,27 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                     __threadfence();
                     if (row_ok) {
                         const float* first = p.ws + (static_cast<size_t>(it.tile) * p.splits * kBM + row_in_tile) * BN;
+                        if constexpr (Cfg::GATED) {
 #pragma unroll 1
-                        for (int c = 0; c < BN / 32; ++c) {
+                            for (int c = 0; c < BN / 64; ++c) {
+                                if (it.n0 / 2 + c * 32 >= p.N) break;
+                                float gate[32], up[32];
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) gate[i] = up[i] = 0.f;
+                                for (int s = 0; s < p.splits; ++s) {
+                                    const float4* src = reinterpret_cast<const float4*>(first + static_cast<size_t>(s) * kBM * BN + c * 32);
+#pragma unroll
+                                    for (int v = 0; v < 8; ++v) {
+                                        const float4 a = __ldcg(src + v), b = __ldcg(src + BN / 8 + v);
+                                        gate[4 * v] += a.x; gate[4 * v + 1] += a.y; gate[4 * v + 2] += a.z; gate[4 * v + 3] += a.w;
+                                        up[4 * v] += b.x; up[4 * v + 1] += b.y; up[4 * v + 2] += b.z; up[4 * v + 3] += b.w;
+                                    }
+                                }
+                                store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, gate, up);
+                            }
+                        }
+#pragma unroll 1
+                        for (int c = 0; c < (Cfg::GATED ? 0 : BN / 32); ++c) {
                             if (it.n0 + c * 32 >= p.N) break;
                             float accv[32];
 #pragma unroll
@@ -1415,6 +1547,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
         constexpr int A_NROW = Cfg::A_MN ? NPIX : A_ITERS, A_NCOL = Cfg::A_MN ? A_ITERS / NPIX : 1;
         constexpr int B_NROW = Cfg::B_MN ? NPIX : B_ITERS, B_NCOL = Cfg::B_MN ? B_ITERS / NPIX : 1;
         static_assert(A_ITERS % NPIX == 0 && B_ITERS % NPIX == 0, "an MN-major tile is whole 128-byte chunks");
+        constexpr int HALF = Cfg::GATED ? B_NCOL / 2 : B_NCOL;  // GATED: 128-byte chunks from HALF on belong to the second stored matrix
         const int r0 = lw * 4 + sub;
         // 16 i + r0 keeps its low three bits, so the swizzled position is that of row r0 plus 2048 i
         const uint32_t sw_a = swz<Cfg::A_B32>(r0, j), sw_b = swz<Cfg::B_B32>(r0, j);
@@ -1446,7 +1579,8 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                 for (int i = 0; i < B_ITERS; ++i) rb[i] = row_state(p.b, it.n0 + 16 * i + r0);
             } else {
 #pragma unroll
-                for (int q = 0; q < B_NCOL; ++q) cb[q] = col_state<Cfg::VEC>(p.b, it.n0 + q * CE + j * Cfg::VEC);
+                for (int q = 0; q < B_NCOL; ++q)
+                    cb[q] = col_state<Cfg::VEC>(p.b, (Cfg::GATED ? it.n0 / 2 + q % HALF * CE : it.n0 + q * CE) + j * Cfg::VEC);
             }
             for (int kk = it.kb_begin; kk < it.kb_end; ++kk, ++t) {
                 if (t % Cfg::LOADER_GROUPS != group) continue;
@@ -1491,7 +1625,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                 for (int i = 0; i < B_ITERS; ++i) {
                     const RowState& r = rb[Cfg::B_MN ? i % NPIX : i];
                     const ColState& k = cb[Cfg::B_MN ? i / NPIX : 0];
-                    uintptr_t addr = chunk_addr<InT>(p.b, base_b, r, k);
+                    uintptr_t addr = chunk_addr<InT>(p.b, base_b + (Cfg::GATED && i / NPIX >= HALF ? p.b.batch_stride : 0), r, k);
                     if (k.how == kChunkSlow) slow |= 1u << (16 + i);
                     vb[i] = ldg_pred(k.how == kChunkFast ? addr : 0);
                 }
@@ -1512,9 +1646,10 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                         int r = 16 * i + r0;
                         int g = Cfg::B_MN ? k0 + (r % BK) : it.n0 + r;
                         int col = Cfg::B_MN ? it.n0 + (r / BK) * CE + j * Cfg::VEC : k0 + j * Cfg::VEC;
+                        if (Cfg::GATED) col = it.n0 / 2 + r / BK % HALF * CE + j * Cfg::VEC;
                         ColCtx kc = {};
                         if (p.b.kind == 1) kc = col_ctx<Cfg::VEC>(p.b, col);
-                        vb[i] = fetch16<InT, Cfg::VEC>(p.b, g, col, boff_b, kc);
+                        vb[i] = fetch16<InT, Cfg::VEC>(p.b, g, col, Cfg::GATED && r / BK >= HALF ? p.b.batch_stride : boff_b, kc);
                     }
                 }
 #pragma unroll

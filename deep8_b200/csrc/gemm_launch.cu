@@ -652,6 +652,104 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
     return 0;
 }
 
+int run_gated(Ctx* ctx, const GatedProblem& g) {
+    const bool f32 = g.dtype == 1;
+    const int esize = f32 ? 4 : 2, bk = 128 / esize;
+    HostOperand a, b;
+    a.ptr = g.a;
+    a.ld = g.K;
+    b.ptr = g.b;
+    b.mn = true;
+    b.ld = g.N;
+    b.batch_count = 2;
+    b.batch_stride = static_cast<long long>(g.K) * g.N;
+    const bool tma = tma_ok(a, esize) && tma_ok(b, esize) && encode_tiled() != nullptr && !env_int("D8K_FORCE_GATHER", 0);
+    const long long mtiles = (g.M + kBM - 1) / kBM, ptiles = (g.M + 255LL) / 256 * ((g.N + 127) / 128);
+    // The paired kernel from half a wave of its tiles on, with a long contraction from a third of one, as in make_plan.
+    const bool pair = tma && !f32 && g.K % 64 == 0 && g.N % 64 == 0 && env_int("D8K_PAIR", 1) != 0 &&
+                      (ptiles * 2 >= ctx->num_sms || (g.K >= 2048 && ptiles * 3 >= ctx->num_sms));
+    int bn = f32 ? 64 : 128;
+    if (!f32 && tma && mtiles * ((g.N + 127) / 128) >= ctx->num_sms) bn = 256;  // wide tiles when they alone give every SM one
+    const long long tiles = pair ? ptiles : mtiles * ((g.N + bn / 2 - 1) / (bn / 2));
+    if (tiles >= (1LL << 30)) return fail(1, "the shape is too large");
+
+    GemmParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.M = g.M; p.N = g.N; p.K = g.K;
+    p.batch = p.kbatch = 1;
+    p.num_kb = (g.K + bk - 1) / bk;
+    p.tiles_m = static_cast<int>(pair ? (g.M + 255LL) / 256 : mtiles);
+    p.tiles_n = static_cast<int>(tiles / p.tiles_m);
+    p.raster_group = 16;
+    int splits = 1;  // as in make_plan: at least 24 k-blocks per split
+    if (!pair && tiles * 2 <= ctx->num_sms && tiles <= kMaxCounters) {
+        splits = ctx->num_sms / static_cast<int>(tiles);
+        if (splits > p.num_kb / 24) splits = p.num_kb / 24;
+        const size_t per_split = static_cast<size_t>(tiles) * kBM * bn * sizeof(float);
+        if (splits > 1 && per_split * splits > ctx->scratch_bytes) splits = static_cast<int>(ctx->scratch_bytes / per_split);
+        if (splits > 255) splits = 255;
+        if (splits < 1) splits = 1;
+    }
+    p.kb_per_split = (p.num_kb + splits - 1) / splits;
+    p.splits = (p.num_kb + p.kb_per_split - 1) / p.kb_per_split;
+    p.total_work = static_cast<int>(tiles) * p.splits;
+    p.C = g.C;
+    p.ldc = g.N;
+    p.gated = g.tail;
+    p.ws = ctx->scratch;
+    p.counters = ctx->counters;
+    p.status = ctx->status;
+    p.a_batch_mod = 1;
+    p.b_batch_mod = 2;
+
+    CUtensorMap ta, tb;
+    std::memset(&ta, 0, sizeof(ta));
+    std::memset(&tb, 0, sizeof(tb));
+    GemmLaunchFn fn = nullptr;
+    int resident = ctx->num_sms;  // work items in flight together
+    const char* form = "gather";
+    if (pair) {
+        if (!make_pair_map(&ta, a, g.M, g.K) || !make_pair_map(&tb, b, g.N, g.K)) return fail(2, "gated: cuTensorMapEncodeTiled (4-D) failed");
+        const Raster r = pick_raster(g.M, 2LL * g.N, g.K, p.tiles_m, p.tiles_n, ctx->num_sms / 2);
+        p.raster_group = r.group;
+        p.raster_n = r.along_n;
+        fn = lookup_f16_gated_pair();
+        resident = ctx->num_sms / 2;
+        form = "pair";
+    } else if (tma) {
+        p.a_tma = p.b_tma = kTmaTiled;
+        p.b_chunked = !f32 && g.N % bk == 0;  // each projection's columns of a tile as one box
+        if (!make_map(&ta, a, g.K, g.M, kBM, esize) ||
+            !(p.b_chunked ? make_pair_map(&tb, b, g.N, g.K, bk, bn / 2 / bk, esize) : make_map(&tb, b, g.N, g.K, bk, esize, f32)))
+            return fail(2, "gated: cuTensorMapEncodeTiled failed");
+        form = "tma";
+        if (f32) {  // two CTAs per SM when there is more than one tile per SM and no split, as in run_gemm
+            const int mode = p.splits == 1 && p.total_work > ctx->num_sms ? (p.num_kb > 8 ? 2 : 1) : 4;
+            fn = lookup_f32_gated(mode);
+            if (mode != 4) {
+                resident = 2 * ctx->num_sms;
+                form = "tma dual";
+            }
+        } else {
+            fn = lookup_f16_gated(bn);
+        }
+    } else {
+        p.a = to_gather(a, g.M, g.K, esize);
+        p.b = to_gather(b, g.K, g.N, esize);
+        fn = lookup_gated_gather(f32);
+    }
+    if (!fn) return fail(2, "gated: no kernel for this configuration");
+    const int grid = p.total_work < resident ? p.total_work : resident;
+    if (p.splits > 1) p.epoch = next_epoch(ctx);
+    cudaError_t e = fn(grid, ctx->stream, ta, tb, p);
+    if (e != cudaSuccess) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
+    count_launch();
+    std::ostringstream os;
+    os << (f32 ? "f32 " : "f16 ") << "gated " << form << " bn=" << (pair ? 256 : bn) << " splits=" << p.splits << " grid=" << grid;
+    set_last_kernel(os.str());
+    return 0;
+}
+
 int run_gemm_group(Ctx* ctx, std::vector<GemmProblem>& parts) {
     const int n = static_cast<int>(parts.size());
     if (n == 0) return 0;
