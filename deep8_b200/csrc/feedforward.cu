@@ -25,158 +25,356 @@ namespace {
     } while (0)
 
 // ------------------------------------------------------------------------------------------------ gated projections
-// dpre from pre and dz, four consecutive elements (one counter of the generator) per step: 5 accesses per element, bound by HBM.
-// pre and dpre may be the same memory (an element is read and written by one thread), so nothing here is declared __restrict__.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const T* dz, T* dpre, size_t n, int act, DropSpec drop, int dropping) {
+// A pack of W consecutive elements as one memory access: 16 bytes, or a single element where rows or bases are not aligned to that.
+template <typename T, int W>
+struct alignas(W * sizeof(T)) Pack {
+    T v[W];
+};
+template <typename T, int W>
+__device__ __forceinline__ Pack<T, W> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, W>*>(p);
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, W>& v) {
+    *reinterpret_cast<Pack<T, W>*>(p) = v;
+}
+
+// dpre from pre and dz: five accesses per element, bound by HBM (8192 x 16384 fp16: 234 us, 5.7 TB/s).  pre and dpre may be the same
+// memory (an element is read and written by one thread), so nothing here is declared __restrict__.
+template <int ACT, typename T, int E>
+__device__ __forceinline__ void gated_grad_elements(Pack<T, E>& g, Pack<T, E>& u, const Pack<T, E>& d, size_t i0, unsigned long long offset, const DropSpec& drop,
+                                                    int dropping) {
     constexpr bool FAST = sizeof(T) == 2;
-    constexpr int V = 16 / sizeof(T);     // elements of a 16-byte access
-    constexpr int E = VEC ? V : 4;        // elements per step
-    const unsigned long long offset = dropping ? drop_offset(drop) : 0;
-    const size_t steps = (n + E - 1) / E;
-    for (size_t s = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; s < steps; s += gridDim.x * static_cast<size_t>(blockDim.x)) {
-        const size_t i0 = s * E;
-        alignas(16) T g[E], u[E], d[E];
-        if (VEC) {
-            *reinterpret_cast<uint4*>(g) = *reinterpret_cast<const uint4*>(pre + i0);
-            *reinterpret_cast<uint4*>(u) = *reinterpret_cast<const uint4*>(pre + n + i0);
-            *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(dz + i0);
-        } else {
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                const bool in = i0 + k < n;
-                g[k] = in ? pre[i0 + k] : narrow<T>(0.0f);
-                u[k] = in ? pre[n + i0 + k] : narrow<T>(0.0f);
-                d[k] = in ? dz[i0 + k] : narrow<T>(0.0f);
-            }
-        }
+    for (int q = 0; q < E / 4; ++q) {
+        uint4 words = make_uint4(0u, 0u, 0u, 0u);
+        if (dropping) words = philox4x32((i0 >> 2) + q, offset, drop.seed);
+        const uint32_t word[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
-        for (int q = 0; q < E / 4; ++q) {
-            uint4 words = make_uint4(0u, 0u, 0u, 0u);
-            if (dropping) words = philox4x32((i0 >> 2) + q, offset, drop.seed);
-            const uint32_t word[4] = {words.x, words.y, words.z, words.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float value, slope;
-                activation<FAST, true>(act, widen(g[4 * q + k]), value, slope);
-                const float dd = dropping ? widen(d[4 * q + k]) * drop.scale : widen(d[4 * q + k]);
-                float dg = dd * widen(u[4 * q + k]) * slope, du = dd * value;
-                if (dropping && !drop_keeps(drop, word[k])) dg = du = 0.0f;
-                g[4 * q + k] = narrow<T>(dg);
-                u[4 * q + k] = narrow<T>(du);
-            }
-        }
-        if (VEC) {
-            *reinterpret_cast<uint4*>(dpre + i0) = *reinterpret_cast<const uint4*>(g);
-            *reinterpret_cast<uint4*>(dpre + n + i0) = *reinterpret_cast<const uint4*>(u);
-        } else {
-#pragma unroll
-            for (int k = 0; k < E; ++k)
-                if (i0 + k < n) {
-                    dpre[i0 + k] = g[k];
-                    dpre[n + i0 + k] = u[k];
-                }
+        for (int k = 0; k < 4; ++k) {
+            float value, slope;
+            activation<ACT, FAST, true>(widen(g.v[4 * q + k]), value, slope);
+            const float dd = dropping ? widen(d.v[4 * q + k]) * drop.scale : widen(d.v[4 * q + k]);
+            float dg = dd * widen(u.v[4 * q + k]) * slope, du = dd * value;
+            if (dropping && !drop_keeps(drop, word[k])) dg = du = 0.0f;  // whatever the projections held
+            g.v[4 * q + k] = narrow<T>(dg);
+            u.v[4 * q + k] = narrow<T>(du);
         }
     }
 }
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const T* dz, T* dpre, size_t n, int act, DropSpec drop, int dropping) {
+    constexpr int E = VEC ? 16 / sizeof(T) : 4;
+    const unsigned long long offset = dropping ? drop_offset(drop) : 0;
+    const size_t steps = (n + E - 1) / E, stride = gridDim.x * static_cast<size_t>(blockDim.x);
+    with_activation(act, [&](auto which) {
+        for (size_t s = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; s < steps; s += stride) {
+            const size_t i0 = s * E;
+            Pack<T, E> g, u, d;
+            if (VEC) {
+                g = load_pack<T, E>(pre + i0);
+                u = load_pack<T, E>(pre + n + i0);
+                d = load_pack<T, E>(dz + i0);
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    const bool in = i0 + k < n;
+                    g.v[k] = in ? pre[i0 + k] : narrow<T>(0.0f);
+                    u.v[k] = in ? pre[n + i0 + k] : narrow<T>(0.0f);
+                    d.v[k] = in ? dz[i0 + k] : narrow<T>(0.0f);
+                }
+            }
+            gated_grad_elements<decltype(which)::value>(g, u, d, i0, offset, drop, dropping);
+            if (VEC) {
+                store_pack(dpre + i0, g);
+                store_pack(dpre + n + i0, u);
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; ++k)
+                    if (i0 + k < n) {
+                        dpre[i0 + k] = g.v[k];
+                        dpre[n + i0 + k] = u.v[k];
+                    }
+            }
+        }
+    });
+}
 
 // ------------------------------------------------------------------------------------------------ dropout
-// y = (residual +) dropout(x): `residual` is the accumulated gradient itself in the backward pass.  Four consecutive elements share one
-// counter of the generator.
-template <typename T, bool VEC>
+// One pack of y = (residual +) dropout(x), i0 the index of its first element (a multiple of four)
+template <typename T, int E>
+__device__ __forceinline__ void drop_pack(Pack<T, E>& a, const Pack<T, E>& b, bool add, size_t i0, unsigned long long offset, const DropSpec& drop) {
+#pragma unroll
+    for (int q = 0; q < E / 4; ++q) {
+        const uint4 words = philox4x32((i0 >> 2) + q, offset, drop.seed);
+        const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float v = drop_keeps(drop, word[k]) ? widen(a.v[4 * q + k]) * drop.scale : 0.0f;
+            if (add) v += widen(b.v[4 * q + k]);
+            a.v[4 * q + k] = narrow<T>(v);
+        }
+    }
+}
+// y = (residual +) dropout(x): `residual` is the accumulated gradient itself in the backward pass.  VEC: bases on 16-byte boundaries; the
+// last, partial pack goes element by element either way.  y may be x or residual, so nothing is declared __restrict__.
+template <typename T, bool VEC, bool ADD>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, T* y, size_t n, DropSpec drop) {
-    constexpr int V = 16 / sizeof(T);
-    constexpr int E = VEC ? V : 4;
+    constexpr int E = VEC ? 16 / sizeof(T) : 4;
     const unsigned long long offset = drop_offset(drop);
-    const size_t steps = (n + E - 1) / E;
-    for (size_t s = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; s < steps; s += gridDim.x * static_cast<size_t>(blockDim.x)) {
-        const size_t i0 = s * E;
-        alignas(16) T a[E], b[E];
-        if (VEC) {
-            *reinterpret_cast<uint4*>(a) = *reinterpret_cast<const uint4*>(x + i0);
-            if (residual) *reinterpret_cast<uint4*>(b) = *reinterpret_cast<const uint4*>(residual + i0);
-        } else {
+    const size_t whole = n / E, stride = gridDim.x * static_cast<size_t>(blockDim.x);
+    size_t s = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x;
+    if (VEC) {
+        constexpr int U = 2;  // packs in flight per thread
+        for (; s + (U - 1) * stride < whole; s += U * stride) {
+            Pack<T, E> a[U], b[U] = {};
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                a[k] = i0 + k < n ? x[i0 + k] : narrow<T>(0.0f);
-                if (residual) b[k] = i0 + k < n ? residual[i0 + k] : narrow<T>(0.0f);
+            for (int k = 0; k < U; ++k) {
+                a[k] = load_pack<T, E>(x + (s + k * stride) * E);
+                if (ADD) b[k] = load_pack<T, E>(residual + (s + k * stride) * E);
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                drop_pack(a[k], b[k], ADD, (s + k * stride) * E, offset, drop);
+                store_pack(y + (s + k * stride) * E, a[k]);
             }
         }
+        for (; s < whole; s += stride) {
+            Pack<T, E> a = load_pack<T, E>(x + s * E), b = {};
+            if (ADD) b = load_pack<T, E>(residual + s * E);
+            drop_pack(a, b, ADD, s * E, offset, drop);
+            store_pack(y + s * E, a);
+        }
+    }
+    for (; s * E < n; s += stride) {
+        Pack<T, E> a = {}, b = {};
 #pragma unroll
-        for (int q = 0; q < E / 4; ++q) {
-            const uint4 words = philox4x32((i0 >> 2) + q, offset, drop.seed);
-            const uint32_t word[4] = {words.x, words.y, words.z, words.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                float v = drop_keeps(drop, word[k]) ? widen(a[4 * q + k]) * drop.scale : 0.0f;
-                if (residual) v += widen(b[4 * q + k]);
-                a[4 * q + k] = narrow<T>(v);
+        for (int k = 0; k < E; ++k)
+            if (s * E + k < n) {
+                a.v[k] = x[s * E + k];
+                if (ADD) b.v[k] = residual[s * E + k];
             }
-        }
-        if (VEC) {
-            *reinterpret_cast<uint4*>(y + i0) = *reinterpret_cast<const uint4*>(a);
-        } else {
+        drop_pack(a, b, ADD, s * E, offset, drop);
 #pragma unroll
-            for (int k = 0; k < E; ++k)
-                if (i0 + k < n) y[i0 + k] = a[k];
-        }
+        for (int k = 0; k < E; ++k)
+            if (s * E + k < n) y[s * E + k] = a.v[k];
     }
 }
 
 // ------------------------------------------------------------------------------------------------ root-mean-square norm
-// Sum over the CTA's 256 threads, the same value in every thread; `part` is 8 floats of shared memory.
-__device__ __forceinline__ float cta_sum(float v, float* part) {
+// Rows are short enough for registers almost always: `tpr` threads (a power of two from 32 on) hold a row as N packs each, so x (and dy)
+// cross from memory once.  A CTA has blockDim.x / tpr rows in work at a time.
+//
+// Sum over the tpr threads of a row, the same value in each of them.  part: 16 floats of shared memory that the previous row's sum does
+// not use (two buffers in turn, one barrier per row).
+__device__ __forceinline__ float row_sum(float v, int tpr, float* part) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();  // the last row's sum has been read
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    if (tpr == 32) return v;
+    const int warp = threadIdx.x >> 5, per = tpr >> 5;
+    if ((threadIdx.x & 31) == 0) part[warp] = v;
     __syncthreads();
+    const int first = warp & ~(per - 1);
     float t = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) t += part[k];
+    for (int k = 0; k < per; ++k) t += part[first + k];
     return t;
 }
 
-// One CTA per row, the row read twice (the second time from cache).  y may be x: nothing is declared __restrict__.
-template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_forward_kernel(const T* x, const T* weight, T* y, float* rstd, size_t rows, int cols, float eps) {
-    __shared__ float part[8];
-    for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
+template <typename T, int W, int N>
+__global__ void __launch_bounds__(512) rms_norm_forward_kernel(const T* x, const T* weight, T* y, float* rstd, size_t rows, int cols, float eps, int tpr) {
+    __shared__ float part[2][16];
+    const int at = threadIdx.x & (tpr - 1), sub = threadIdx.x / tpr, group = blockDim.x / tpr;
+    const int packs = cols / W;
+    int buf = 0;
+    for (size_t r0 = blockIdx.x * static_cast<size_t>(group); r0 < rows; r0 += gridDim.x * static_cast<size_t>(group), buf ^= 1) {
+        const size_t r = r0 + sub;
+        const bool live = r < rows;
         const T* row = x + r * cols;
+        Pack<T, W> v[N];
         float sum = 0.0f;
-        for (int c = threadIdx.x; c < cols; c += 256) {
-            const float v = widen(row[c]);
-            sum = fmaf(v, v, sum);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int i = at + k * tpr;
+            v[k] = Pack<T, W>{};
+            if (live && i < packs) v[k] = load_pack<T, W>(row + static_cast<size_t>(i) * W);
         }
-        sum = cta_sum(sum, part);
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum = fmaf(widen(v[k].v[j]), widen(v[k].v[j]), sum);
+        sum = row_sum(sum, tpr, part[buf]);
         const float inv = 1.0f / sqrtf(sum / cols + eps);
-        if (rstd && threadIdx.x == 0) rstd[r] = inv;
-        for (int c = threadIdx.x; c < cols; c += 256) y[r * cols + c] = narrow<T>(widen(row[c]) * inv * widen(weight[c]));
+        if (live && rstd && at == 0) rstd[r] = inv;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int i = at + k * tpr;
+            if (live && i < packs) {
+                const Pack<T, W> w = load_pack<T, W>(weight + static_cast<size_t>(i) * W);
+#pragma unroll
+                for (int j = 0; j < W; ++j) v[k].v[j] = narrow<T>(widen(v[k].v[j]) * inv * widen(w.v[j]));
+                store_pack(y + r * cols + static_cast<size_t>(i) * W, v[k]);
+            }
+        }
     }
 }
 
+// dx (+)= and this CTA's part of dweight (partial[blockIdx.x][cols]) in one pass over x and dy: the columns a thread holds are the same for
+// every row, so their sums stay in its registers.  The next row's loads are issued before this row's sum is formed.
+template <typename T, int W, int N>
+__global__ void __launch_bounds__(512) rms_norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ weight, const float* __restrict__ rstd,
+                                                                T* dx, float* __restrict__ partial, const T* __restrict__ dy, size_t rows, int cols,
+                                                                int accumulate, int tpr) {
+    extern __shared__ float columns[];  // (group - 1) x cols, only for several rows at a time
+    __shared__ float part[2][16];
+    const int at = threadIdx.x & (tpr - 1), sub = threadIdx.x / tpr, group = blockDim.x / tpr;
+    const int packs = cols / W;
+    const size_t step = gridDim.x * static_cast<size_t>(group);
+    float dw[N][W];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+        for (int j = 0; j < W; ++j) dw[k][j] = 0.0f;
+    Pack<T, W> xs[N], gs[N];
+    float inv = 0.0f;
+    auto fetch = [&](size_t r) {
+        const bool live = r < rows;
+        inv = live ? rstd[r] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int i = at + k * tpr;
+            xs[k] = gs[k] = Pack<T, W>{};
+            if (live && i < packs) {
+                xs[k] = load_pack<T, W>(x + r * cols + static_cast<size_t>(i) * W);
+                gs[k] = load_pack<T, W>(dy + r * cols + static_cast<size_t>(i) * W);
+            }
+        }
+    };
+    fetch(blockIdx.x * static_cast<size_t>(group) + sub);
+    int buf = 0;
+    for (size_t r0 = blockIdx.x * static_cast<size_t>(group); r0 < rows; r0 += step, buf ^= 1) {
+        const size_t r = r0 + sub;
+        const float scale = inv;
+        float n[N][W], u[N][W], sum = 0.0f;  // x * rstd, dy * weight
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int i = at + k * tpr;
+            Pack<T, W> w = {};
+            if (i < packs) w = load_pack<T, W>(weight + static_cast<size_t>(i) * W);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float g = widen(gs[k].v[j]);
+                n[k][j] = widen(xs[k].v[j]) * scale;
+                u[k][j] = g * widen(w.v[j]);
+                dw[k][j] = fmaf(g, n[k][j], dw[k][j]);
+                sum = fmaf(u[k][j], n[k][j], sum);
+            }
+        }
+        if (r0 + step < rows) fetch(r + step);
+        if (!dx) continue;
+        const float mean = row_sum(sum, tpr, part[buf]) / cols;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int i = at + k * tpr;
+            if (r < rows && i < packs) {
+                T* dst = dx + r * cols + static_cast<size_t>(i) * W;
+                Pack<T, W> out = {};
+                if (accumulate) out = load_pack<T, W>(dst);
+#pragma unroll
+                for (int j = 0; j < W; ++j) out.v[j] = narrow<T>(fmaf(scale, u[k][j] - n[k][j] * mean, accumulate ? widen(out.v[j]) : 0.0f));
+                store_pack(dst, out);
+            }
+        }
+    }
+    if (!partial) return;
+    // the CTA's rows meet in shared memory, in order
+    if (sub > 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int i = at + k * tpr;
+            if (i < packs)
+#pragma unroll
+                for (int j = 0; j < W; ++j) columns[static_cast<size_t>(sub - 1) * cols + i * W + j] = dw[k][j];
+        }
+    }
+    if (group > 1) __syncthreads();
+    if (sub == 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int i = at + k * tpr;
+            if (i < packs) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    float t = dw[k][j];
+                    for (int g = 1; g < group; ++g) t += columns[static_cast<size_t>(g - 1) * cols + i * W + j];
+                    partial[static_cast<size_t>(blockIdx.x) * cols + i * W + j] = t;
+                }
+            }
+        }
+    }
+}
+
+// dweight (+)= the slices of `partial` in order: 32 columns per CTA, 32 warps that take slices w, w + 32, ... and meet in shared memory in
+// warp order - a single thread per column spent one memory latency after another (39 us for 444 slices).
 template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_grad_x_kernel(const T* __restrict__ x, const T* __restrict__ weight, const float* __restrict__ rstd,
-                                                              T* __restrict__ dx, const T* __restrict__ dy, size_t rows, int cols, int accumulate) {
-    __shared__ float part[8];
-    for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
+__global__ void __launch_bounds__(1024) rms_norm_grad_w_final_kernel(T* __restrict__ dweight, const float* __restrict__ partial, int slices, int cols,
+                                                                     int accumulate) {
+    __shared__ float part[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    float sum = 0.0f;
+    if (c < cols) {
+#pragma unroll 8
+        for (int s = warp; s < slices; s += 32) sum += partial[static_cast<size_t>(s) * cols + c];
+    }
+    part[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && c < cols) {
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) t += part[k][lane];
+        dweight[c] = narrow<T>(accumulate ? widen(dweight[c]) + t : t);
+    }
+}
+
+// Rows too long for registers (above 16384 fp16 or 8192 fp32 columns in 16-byte packs, 8192 otherwise): one CTA per row, the row read twice,
+// the second time from cache.
+template <typename T>
+__global__ void __launch_bounds__(512) rms_norm_forward_long_kernel(const T* x, const T* weight, T* y, float* rstd, size_t rows, int cols, float eps) {
+    __shared__ float part[2][16];
+    int buf = 0;
+    for (size_t r = blockIdx.x; r < rows; r += gridDim.x, buf ^= 1) {
+        const T* row = x + r * cols;
+        float sum = 0.0f;
+        for (int c = threadIdx.x; c < cols; c += 512) {
+            const float v = widen(row[c]);
+            sum = fmaf(v, v, sum);
+        }
+        sum = row_sum(sum, 512, part[buf]);
+        const float inv = 1.0f / sqrtf(sum / cols + eps);
+        if (rstd && threadIdx.x == 0) rstd[r] = inv;
+        for (int c = threadIdx.x; c < cols; c += 512) y[r * cols + c] = narrow<T>(widen(row[c]) * inv * widen(weight[c]));
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(512) rms_norm_grad_x_long_kernel(const T* __restrict__ x, const T* __restrict__ weight, const float* __restrict__ rstd,
+                                                                   T* __restrict__ dx, const T* __restrict__ dy, size_t rows, int cols, int accumulate) {
+    __shared__ float part[2][16];
+    int buf = 0;
+    for (size_t r = blockIdx.x; r < rows; r += gridDim.x, buf ^= 1) {
         const size_t at = r * cols;
         const float inv = rstd[r];
         float sum = 0.0f;
-        for (int c = threadIdx.x; c < cols; c += 256) sum = fmaf(widen(dy[at + c]) * widen(weight[c]), widen(x[at + c]) * inv, sum);
-        const float mean = cta_sum(sum, part) / cols;
-        for (int c = threadIdx.x; c < cols; c += 256) {
+        for (int c = threadIdx.x; c < cols; c += 512) sum = fmaf(widen(dy[at + c]) * widen(weight[c]), widen(x[at + c]) * inv, sum);
+        const float mean = row_sum(sum, 512, part[buf]) / cols;
+        for (int c = threadIdx.x; c < cols; c += 512) {
             float v = inv * (widen(dy[at + c]) * widen(weight[c]) - widen(x[at + c]) * inv * mean);
             if (accumulate) v += widen(dx[at + c]);
             dx[at + c] = narrow<T>(v);
         }
     }
 }
-
-// Column sums of dy * x * rstd in two fixed-order steps: a thread per column and slice of rows, then the slices in order.
 template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_grad_w_kernel(const T* __restrict__ x, const float* __restrict__ rstd, const T* __restrict__ dy,
-                                                              float* __restrict__ partial, size_t rows, int cols, size_t rows_per_slice) {
+__global__ void __launch_bounds__(256) rms_norm_grad_w_long_kernel(const T* __restrict__ x, const float* __restrict__ rstd, const T* __restrict__ dy,
+                                                                   float* __restrict__ partial, size_t rows, int cols, size_t rows_per_slice) {
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= cols) return;
     const size_t r0 = blockIdx.y * rows_per_slice;
@@ -184,15 +382,6 @@ __global__ void __launch_bounds__(256) rms_norm_grad_w_kernel(const T* __restric
     float sum = 0.0f;
     for (size_t r = r0; r < r1; ++r) sum = fmaf(widen(dy[r * cols + c]), widen(x[r * cols + c]) * rstd[r], sum);
     partial[static_cast<size_t>(blockIdx.y) * cols + c] = sum;
-}
-template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_grad_w_final_kernel(T* __restrict__ dweight, const float* __restrict__ partial, int slices, int cols,
-                                                                    int accumulate) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= cols) return;
-    float sum = 0.0f;
-    for (int s = 0; s < slices; ++s) sum += partial[static_cast<size_t>(s) * cols + c];
-    dweight[c] = narrow<T>(accumulate ? widen(dweight[c]) + sum : sum);
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -372,11 +561,12 @@ int dropout(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* 
     if ((y != x && overlap(y, bytes, x, bytes)) || (y != residual && overlap(y, bytes, residual, bytes)))
         return fail(D8K_ERR_ARGUMENT, "dropout: the output overlaps an input");
     const int per = static_cast<int>(16 / esize(dtype));
-    const bool vec = aligned16({x, residual, y}) && n % per == 0;
+    const bool vec = aligned16({x, residual, y});
     const int grid = grid_for(ctx, (n + per - 1) / (vec ? per : 4));
     auto run = [&](auto zero) {
         using T = decltype(zero);
-        auto kernel = vec ? dropout_kernel<T, true> : dropout_kernel<T, false>;
+        auto kernel = residual ? (vec ? dropout_kernel<T, true, true> : dropout_kernel<T, false, true>)
+                               : (vec ? dropout_kernel<T, true, false> : dropout_kernel<T, false, false>);
         kernel<<<grid, 256, 0, ctx->stream>>>(static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<T*>(y), n, spec);
     };
     if (dtype == D8K_F32) run(0.0f);
@@ -386,27 +576,90 @@ int dropout(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* 
     return 0;
 }
 
+// How a row of `packs` packs is spread over threads.  The register kernels hold 1, 2 or 4 packs per thread (1, 4 or 16 single elements);
+// `start` is the count to begin with when there are rows enough to fill the GPU, one pack per thread and more threads per row
+// otherwise, because then latency counts.  packs_per_thread == 0: too long for registers.
+struct RowPlan {
+    int tpr, packs_per_thread, threads, group;
+};
+RowPlan plan_rows(const d8k_ctx* ctx, size_t rows, int packs, bool vec, int start) {
+    for (int n = rows < static_cast<size_t>(ctx->num_sms) * 4 ? 1 : start; n <= (vec ? 4 : 16); n *= vec ? 2 : 4) {
+        int tpr = 32;
+        while (tpr < 512 && static_cast<long long>(tpr) * n < packs) tpr *= 2;
+        if (static_cast<long long>(tpr) * n < packs) continue;
+        const int threads = tpr > 256 ? tpr : 256;
+        return RowPlan{tpr, n, threads, threads / tpr};
+    }
+    return RowPlan{0, 0, 0, 0};
+}
+
+template <typename T>
+int rms_norm_forward(d8k_ctx* ctx, const T* x, const T* weight, float eps, T* y, float* rstd, size_t rows, int cols) {
+    constexpr int W = 16 / sizeof(T);
+    const bool vec = aligned16({x, weight, y}) && cols % W == 0;
+    const RowPlan p = plan_rows(ctx, rows, vec ? cols / W : cols, vec, 4);
+    if (p.packs_per_thread == 0) {
+        const size_t cap = static_cast<size_t>(ctx->num_sms) * 4;
+        rms_norm_forward_long_kernel<T><<<static_cast<unsigned>(rows < cap ? rows : cap), 512, 0, ctx->stream>>>(x, weight, y, rstd, rows, cols, eps);
+    } else {
+        const size_t groups = (rows + p.group - 1) / p.group, cap = static_cast<size_t>(ctx->num_sms) * (2048 / p.threads);
+        auto kernel = vec ? (p.packs_per_thread == 1 ? rms_norm_forward_kernel<T, W, 1> : p.packs_per_thread == 2 ? rms_norm_forward_kernel<T, W, 2>
+                                                                                                            : rms_norm_forward_kernel<T, W, 4>)
+                          : (p.packs_per_thread == 1 ? rms_norm_forward_kernel<T, 1, 1> : p.packs_per_thread == 4 ? rms_norm_forward_kernel<T, 1, 4>
+                                                                                                            : rms_norm_forward_kernel<T, 1, 16>);
+        kernel<<<static_cast<unsigned>(groups < cap ? groups : cap), p.threads, 0, ctx->stream>>>(x, weight, y, rstd, rows, cols, eps, p.tpr);
+    }
+    D8K_CUDA(cudaGetLastError());
+    count_launch();
+    return 0;
+}
+
 template <typename T>
 int rms_norm_backward(d8k_ctx* ctx, const T* x, const T* weight, const float* rstd, T* dx, T* dweight, const T* dy, size_t rows, int cols, int accumulate) {
-    if (dweight) {
-        const int strips = (cols + 255) / 256;
-        size_t slices = (static_cast<size_t>(ctx->num_sms) * 8 + strips - 1) / strips;
-        const size_t most = ctx->scratch_bytes / (static_cast<size_t>(cols) * sizeof(float));
-        if (most < 1) return fail(D8K_ERR_ARGUMENT, "the context's scratch memory is smaller than one row of floats");
-        if (slices > most) slices = most;
-        if (slices > (rows + 7) / 8) slices = (rows + 7) / 8;
-        const size_t per = (rows + slices - 1) / slices;
-        slices = (rows + per - 1) / per;
-        rms_norm_grad_w_kernel<T><<<dim3(strips, static_cast<unsigned>(slices)), 256, 0, ctx->stream>>>(x, rstd, dy, ctx->scratch, rows, cols, per);
-        D8K_CUDA(cudaGetLastError());
-        rms_norm_grad_w_final_kernel<T><<<strips, 256, 0, ctx->stream>>>(dweight, ctx->scratch, static_cast<int>(slices), cols, accumulate);
+    constexpr int W = 16 / sizeof(T);
+    const bool vec = aligned16({x, weight, dx, dy}) && cols % W == 0;
+    const RowPlan p = plan_rows(ctx, rows, vec ? cols / W : cols, vec, vec ? 2 : 4);
+    const size_t most = ctx->scratch_bytes / (static_cast<size_t>(cols) * sizeof(float));  // slices of column sums the scratch memory holds
+    if (dweight && most < 1) return fail(D8K_ERR_ARGUMENT, "the context's scratch memory is smaller than one row of floats");
+    if (!dx && !dweight) return 0;
+    size_t slices = 0;
+    if (p.packs_per_thread > 0) {
+        const size_t groups = (rows + p.group - 1) / p.group;
+        auto kernel = vec ? (p.packs_per_thread == 1 ? rms_norm_backward_kernel<T, W, 1> : p.packs_per_thread == 2 ? rms_norm_backward_kernel<T, W, 2>
+                                                                                                             : rms_norm_backward_kernel<T, W, 4>)
+                          : (p.packs_per_thread == 1 ? rms_norm_backward_kernel<T, 1, 1> : p.packs_per_thread == 4 ? rms_norm_backward_kernel<T, 1, 4>
+                                                                                                             : rms_norm_backward_kernel<T, 1, 16>);
+        const size_t dyn = dweight ? static_cast<size_t>(p.group - 1) * cols * sizeof(float) : 0;
+        int per_sm = 0;
+        D8K_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, p.threads, dyn));
+        slices = static_cast<size_t>(ctx->num_sms) * (per_sm < 1 ? 1 : per_sm);
+        if (slices > groups) slices = groups;
+        if (dweight && slices > most) slices = most;
+        kernel<<<static_cast<unsigned>(slices), p.threads, dyn, ctx->stream>>>(x, weight, rstd, dx, dweight ? ctx->scratch : nullptr, dy, rows, cols, accumulate,
+                                                                              p.tpr);
         D8K_CUDA(cudaGetLastError());
         count_launch();
-        count_launch();
+    } else {
+        if (dweight) {
+            const int strips = (cols + 255) / 256;
+            slices = (static_cast<size_t>(ctx->num_sms) * 8 + strips - 1) / strips;
+            if (slices > most) slices = most;
+            if (slices > (rows + 7) / 8) slices = (rows + 7) / 8;
+            const size_t per = (rows + slices - 1) / slices;
+            slices = (rows + per - 1) / per;
+            rms_norm_grad_w_long_kernel<T><<<dim3(strips, static_cast<unsigned>(slices)), 256, 0, ctx->stream>>>(x, rstd, dy, ctx->scratch, rows, cols, per);
+            D8K_CUDA(cudaGetLastError());
+            count_launch();
+        }
+        if (dx) {
+            const size_t cap = static_cast<size_t>(ctx->num_sms) * 4;
+            rms_norm_grad_x_long_kernel<T><<<static_cast<unsigned>(rows < cap ? rows : cap), 512, 0, ctx->stream>>>(x, weight, rstd, dx, dy, rows, cols, accumulate);
+            D8K_CUDA(cudaGetLastError());
+            count_launch();
+        }
     }
-    if (dx) {
-        const size_t cap = static_cast<size_t>(ctx->num_sms) * 8;
-        rms_norm_grad_x_kernel<T><<<static_cast<unsigned>(rows < cap ? rows : cap), 256, 0, ctx->stream>>>(x, weight, rstd, dx, dy, rows, cols, accumulate);
+    if (dweight) {
+        rms_norm_grad_w_final_kernel<T><<<(cols + 31) / 32, 1024, 0, ctx->stream>>>(dweight, ctx->scratch, static_cast<int>(slices), cols, accumulate);
         D8K_CUDA(cudaGetLastError());
         count_launch();
     }
@@ -499,18 +752,9 @@ int d8k_rms_norm_forward(d8k_ctx* ctx, int dtype, const void* x, const void* wei
         if ((y != x && overlap(y, bytes, x, bytes)) || overlap(y, bytes, weight, wbytes) || overlap(rstd, rbytes, x, bytes) || overlap(rstd, rbytes, y, bytes) ||
             overlap(rstd, rbytes, weight, wbytes))
             return fail(D8K_ERR_ARGUMENT, "rms_norm: an output overlaps an input");
-        const size_t cap = static_cast<size_t>(ctx->num_sms) * 8;
-        const unsigned grid = static_cast<unsigned>(rows < cap ? rows : cap);
-        auto run = [&](auto zero) {
-            using T = decltype(zero);
-            rms_norm_forward_kernel<T><<<grid, 256, 0, ctx->stream>>>(static_cast<const T*>(x), static_cast<const T*>(weight), static_cast<T*>(y), rstd,
-                                                                      rows, cols, eps);
-        };
-        if (dtype == D8K_F32) run(0.0f);
-        else run(__half());
-        D8K_CUDA(cudaGetLastError());
-        count_launch();
-        return 0;
+        if (dtype == D8K_F32)
+            return rms_norm_forward<float>(ctx, static_cast<const float*>(x), static_cast<const float*>(weight), eps, static_cast<float*>(y), rstd, rows, cols);
+        return rms_norm_forward<__half>(ctx, static_cast<const __half*>(x), static_cast<const __half*>(weight), eps, static_cast<__half*>(y), rstd, rows, cols);
     });
 }
 

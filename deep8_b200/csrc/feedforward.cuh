@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace d8k {
 
@@ -23,28 +24,41 @@ __device__ __forceinline__ float sigmoid_of(float a) {
 // value = act(a); slope = act'(a) when wanted.  gelu goes through erfc, gelu_tanh through a sigmoid ((1 + tanh z) / 2 = sigmoid(2 z)):
 // both forms keep the relative accuracy of the negative tail, where 1 + erf and 1 + tanh cancel.  Arguments beyond +-80 take the
 // limits' values (an fp16 projection may have overflowed to an infinity, and infinity times a vanished factor would be a NaN).
-template <bool FAST, bool SLOPE>
-__device__ __forceinline__ void activation(int act, float a, float& value, float& slope) {
+template <int ACT, bool FAST, bool SLOPE>
+__device__ __forceinline__ void activation(float a, float& value, float& slope) {
     const float lo = a < -80.0f ? -80.0f : a;
     const float b = lo > 80.0f ? 80.0f : lo;
-    if (act == kActSilu || act == kActSigmoid) {
+    if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
         const float s = sigmoid_of<FAST>(a);
         const float ds = s * (1.0f - s);
-        value = act == kActSilu ? lo * s : s;
-        if (SLOPE) slope = act == kActSilu ? fmaf(b, ds, s) : ds;
-    } else if (act == kActGeluTanh) {
+        value = ACT == kActSilu ? lo * s : s;
+        if (SLOPE) slope = ACT == kActSilu ? fmaf(b, ds, s) : ds;
+    } else if constexpr (ACT == kActGeluTanh) {
         const float c2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
         const float b2 = b * b;
         const float s = sigmoid_of<FAST>(c2 * b * fmaf(0.044715f, b2, 1.0f));
         value = lo * s;
         if (SLOPE) slope = fmaf(b * s * (1.0f - s), c2 * fmaf(0.134145f, b2, 1.0f), s);
-    } else if (act == kActGelu) {
+    } else if constexpr (ACT == kActGelu) {
         const float cdf = 0.5f * erfcf(-0.7071067811865476f * b);
         value = lo * cdf;
         if (SLOPE) slope = fmaf(b * 0.3989422804014327f, FAST ? __expf(-0.5f * b * b) : expf(-0.5f * b * b), cdf);
     } else {  // relu: a NaN gives 0, as in the framework's ReLU
         value = a > 0.0f ? a : 0.0f;
         if (SLOPE) slope = a > 0.0f ? 1.0f : 0.0f;
+    }
+}
+
+// f(std::integral_constant<int, act>): one branch around a whole group of elements.  A branch per element would keep the compiler from
+// overlapping the elements' exponentials and divisions, and an epilogue has too few warps to hide them otherwise.
+template <class F>
+__device__ __forceinline__ void with_activation(int act, F f) {
+    switch (act) {
+        case kActSilu: f(std::integral_constant<int, kActSilu>()); break;
+        case kActGelu: f(std::integral_constant<int, kActGelu>()); break;
+        case kActGeluTanh: f(std::integral_constant<int, kActGeluTanh>()); break;
+        case kActRelu: f(std::integral_constant<int, kActRelu>()); break;
+        default: f(std::integral_constant<int, kActSigmoid>()); break;
     }
 }
 

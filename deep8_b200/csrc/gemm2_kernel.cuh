@@ -44,11 +44,15 @@ struct Gemm2Cfg {
     static constexpr int B_BYTES = HALF_N * 128 * SUB;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;  // per CTA
     static constexpr int TMEM_COLS = 512;        // two accumulator buffers of 256 columns
-    static constexpr int EPI_WARPS = 4, PRODUCER_WARP = 4, MMA_WARP = 5;
-    static constexpr int THREADS = 32 * 6;
+    // GATED: eight epilogue warps (0-3 and 6-9), two for each quarter of the accumulator's rows, each half of the columns: the activation
+    // makes the epilogue several times longer than a plain store, and with four warps it outlasted a K = 4096 tile's main loop
+    static constexpr int EPI_WARPS = GATED ? 8 : 4, PRODUCER_WARP = 4, MMA_WARP = 5;
+    static constexpr int THREADS = 32 * (EPI_WARPS + 2);
     static constexpr int BAR_BYTES = 256;
     // epilogue staging: per epilogue warp three slots (C, E1, E2) of 32 rows x 64 bytes (32 fp16 columns)
-    static constexpr int SLOT_BYTES = 32 * 64, STAGING_BYTES = EPI_WARPS * 3 * SLOT_BYTES;
+    // (GATED: two slots, used in turn)
+    static constexpr int SLOTS = GATED ? 2 : 3;
+    static constexpr int SLOT_BYTES = 32 * 64, STAGING_BYTES = EPI_WARPS * SLOTS * SLOT_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + BAR_BYTES + STAGING_BYTES + 1024;
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
     static_assert(SMEM_BYTES > 114 * 1024, "one CTA per SM");
@@ -313,14 +317,14 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 p.prof[blockIdx.x * 8 + 4] = waited_tmem;
             }
         }
-    } else if (warp < Cfg::EPI_WARPS) {
+    } else if (warp < 4 || Cfg::GATED) {
         // ============================================================================ epilogue (both CTAs, own rows)
         using OutT = __half;
-        const int quarter = warp;
+        const int quarter = warp & 3;  // the accumulator lanes this warp may read
         const int row_in_tile = quarter * 32 + lane;
         const uint32_t tempty_leader0 = ptx::map_to_rank(tempty_bar(0), 0);
         const uint32_t tempty_leader1 = ptx::map_to_rank(tempty_bar(1), 0);
-        const uint32_t staging = bar_base + Cfg::BAR_BYTES + warp * (3 * Cfg::SLOT_BYTES);
+        const uint32_t staging = bar_base + Cfg::BAR_BYTES + (warp < 4 ? warp : warp - 2) * (Cfg::SLOTS * Cfg::SLOT_BYTES);
         // whole 16-byte pieces everywhere: bases, pitch and batch stride multiples of 8 elements
         const bool coalesced = ((reinterpret_cast<uintptr_t>(p.C) | (p.epi ? reinterpret_cast<uintptr_t>(p.E1) : 0) |
                                  (p.epi == 2 ? reinterpret_cast<uintptr_t>(p.E2) : 0)) & 15) == 0 &&
@@ -377,56 +381,62 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             ptx::tc_fence_after_sync();
             const uint32_t taddr = tmem_base + acc * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
             if constexpr (Cfg::GATED) {
-                // 32 columns of both projections at a time; h and, when kept, the projections cross to whole row segments through
-                // the warp's three staging slots
+                // 32 columns of both projections at a time; the projections (when kept) and then h cross to whole row segments through
+                // the warp's two staging slots
                 const GatedTail& t = p.gated;
                 const bool segments = ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(t.pre)) & 15) == 0 && (p.ldc & 7) == 0 && (t.pre_stride & 7) == 0;
+                const int c_begin = warp < 4 ? 0 : 2;
 #pragma unroll 1
-                for (int c = 0; c < 128 / 32; ++c) {
-                    uint32_t r[32], u[32];
-                    __syncwarp();
-                    ptx::tmem_ld_32x32(taddr + c * 32, r);
-                    ptx::tmem_ld_32x32(taddr + 128 + c * 32, u);
-                    ptx::tmem_ld_wait();
+                for (int c = c_begin; c < c_begin + 2; ++c) {
+                    float gate[32], up[32];
+                    {
+                        uint32_t r[32], u[32];
+                        __syncwarp();
+                        ptx::tmem_ld_32x32(taddr + c * 32, r);
+                        ptx::tmem_ld_32x32(taddr + 128 + c * 32, u);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            gate[i] = __uint_as_float(r[i]);
+                            up[i] = __uint_as_float(u[i]);
+                        }
+                    }
                     const int col0 = it.n0 / 2 + c * 32;
                     if (col0 >= p.N) continue;
-                    float gate[32], up[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        gate[i] = __uint_as_float(r[i]);
-                        up[i] = __uint_as_float(u[i]);
-                    }
                     if (!segments || col0 + 32 > p.N) {
                         if (row < p.M) store_gated_chunk<OutT>(p, row, col0, gate, up);
                         continue;
                     }
-                    const uint32_t s0 = staging, s1 = staging + Cfg::SLOT_BYTES, s2 = staging + 2 * Cfg::SLOT_BYTES;
+                    const uint32_t s0 = staging, s1 = staging + Cfg::SLOT_BYTES;
                     using V = EpiVec<OutT>;
-                    const uint32_t stays =
-                        t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0) : 0xffffffffu;
+                    const long long first = static_cast<long long>(warp_row0) * p.ldc + col0 + lc * 8;  // this thread's piece of the segments
+                    if (t.pre) {
 #pragma unroll
-                    for (int v = 0; v < 4; ++v) {
-                        float h[8];
-                        if (t.pre) {
-                            st_shared_v4(s1 + slot_off(lane, v), V::pack(gate + 8 * v));
-                            st_shared_v4(s2 + slot_off(lane, v), V::pack(up + 8 * v));
+                        for (int v = 0; v < 4; ++v) {
+                            st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
+                            st_shared_v4(s1 + slot_off(lane, v), V::pack(up + 8 * v));
                         }
+                        __syncwarp();
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) h[i] = gated_value<OutT>(t, gate[8 * v + i], up[8 * v + i], stays >> (8 * v + i) & 1u);
-                        st_shared_v4(s0 + slot_off(lane, v), V::pack(h));
+                        for (int i = 0; i < 4; ++i) {
+                            const int rr = 8 * i + lr;
+                            if (warp_row0 + rr < p.M) {
+                                OutT* dst = reinterpret_cast<OutT*>(t.pre) + first + static_cast<long long>(rr) * p.ldc;
+                                *reinterpret_cast<uint4*>(dst) = ptx::ld_shared_v4(s0 + slot_off(rr, lc));
+                                *reinterpret_cast<uint4*>(dst + t.pre_stride) = ptx::ld_shared_v4(s1 + slot_off(rr, lc));
+                            }
+                        }
+                        __syncwarp();
                     }
+                    gated_values<OutT>(t, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0, gate, up);
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
                     __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int rr = 8 * i + lr;
-                        if (warp_row0 + rr < p.M) {
-                            const long long e = static_cast<long long>(warp_row0 + rr) * p.ldc + col0 + lc * 8;
-                            *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(p.C) + e) = ptx::ld_shared_v4(s0 + slot_off(rr, lc));
-                            if (t.pre) {
-                                *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(t.pre) + e) = ptx::ld_shared_v4(s1 + slot_off(rr, lc));
-                                *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(t.pre) + t.pre_stride + e) = ptx::ld_shared_v4(s2 + slot_off(rr, lc));
-                            }
-                        }
+                        if (warp_row0 + rr < p.M)
+                            *reinterpret_cast<uint4*>(reinterpret_cast<OutT*>(p.C) + first + static_cast<long long>(rr) * p.ldc) = ptx::ld_shared_v4(s0 + slot_off(rr, lc));
                     }
                 }
             }

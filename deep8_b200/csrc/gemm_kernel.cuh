@@ -791,28 +791,39 @@ __device__ __forceinline__ void store_row_chunk(const GemmParams& p, long long o
 __device__ __forceinline__ uint32_t drop_mask32(const DropSpec& d, unsigned long long first) {
     const unsigned long long offset = drop_offset(d), group = first >> 2;
     const int skip = static_cast<int>(first & 3);
-    unsigned long long bits = 0;
-#pragma unroll 1
-    for (int g = 0; g < (skip ? 9 : 8); ++g) {
+    auto four = [&](int g) -> uint32_t {
         const uint4 w = philox4x32(group + g, offset, d.seed);
-        const unsigned long long four = (drop_keeps(d, w.x) ? 1u : 0u) | (drop_keeps(d, w.y) ? 2u : 0u) | (drop_keeps(d, w.z) ? 4u : 0u) | (drop_keeps(d, w.w) ? 8u : 0u);
-        bits |= four << (4 * g);
+        return (drop_keeps(d, w.x) ? 1u : 0u) | (drop_keeps(d, w.y) ? 2u : 0u) | (drop_keeps(d, w.z) ? 4u : 0u) | (drop_keeps(d, w.w) ? 8u : 0u);
+    };
+    uint32_t bits = 0;
+#pragma unroll 4
+    for (int g = 0; g < 8; ++g) bits |= four(g) << (4 * g);  // four independent chains of ten rounds at a time
+    if (skip) bits = __funnelshift_r(bits, four(8), skip);
+    return bits;
+}
+
+// gate[i] = dropout(act(gate[i]) * up[i]) for 32 consecutive elements, the first of them element `first` of h
+template <typename OutT>
+__device__ __forceinline__ void gated_values(const GatedTail& t, unsigned long long first, float* gate, const float* up) {
+    with_activation(t.act, [&](auto act) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            float value, slope;
+            activation<decltype(act)::value, sizeof(OutT) == 2, false>(gate[i], value, slope);
+            gate[i] = value * up[i];
+        }
+    });
+    if (t.dropping) {
+        const uint32_t stays = drop_mask32(t.drop, first);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) gate[i] = (stays >> i & 1u) ? gate[i] * t.drop.scale : 0.0f;
     }
-    return static_cast<uint32_t>(bits >> skip);
 }
 
-// h of one element from the accumulated projections; `stays`: the dropout's decision (true without one)
+// Tail of a gated product for one row and 32 columns [col0, col0 + 32), clipped to N: both projections (when kept) and h, each rounded
+// once.  Overwrites gate.
 template <typename OutT>
-__device__ __forceinline__ float gated_value(const GatedTail& t, float gate, float up, bool stays) {
-    float value, slope;
-    activation<sizeof(OutT) == 2, false>(t.act, gate, value, slope);
-    const float h = value * up;
-    return t.dropping ? (stays ? h * t.drop.scale : 0.0f) : h;
-}
-
-// Tail of a gated product for one row and 32 columns [col0, col0 + 32), clipped to N: both projections (when kept) and h, each rounded once.
-template <typename OutT>
-__device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, int col0, const float* gate, const float* up) {
+__device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, int col0, float* gate, const float* up) {
     using V = EpiVec<OutT>;
     constexpr int VEC = V::N;
     const GatedTail& t = p.gated;
@@ -820,32 +831,23 @@ __device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, 
     OutT* h = reinterpret_cast<OutT*>(p.C) + off;
     OutT* pg = t.pre ? reinterpret_cast<OutT*>(t.pre) + off : nullptr;
     OutT* pu = t.pre ? pg + t.pre_stride : nullptr;
-    const uint32_t stays = t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(off)) : 0xffffffffu;
     const bool vec_ok = col0 + 32 <= p.N && ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(pg) | reinterpret_cast<uintptr_t>(pu)) & 15) == 0;
-    if (vec_ok) {
+    auto store = [&](OutT* dst, const float* v) {
+        if (vec_ok) {
 #pragma unroll
-        for (int v = 0; v < 32 / VEC; ++v) {
-            float out[VEC];
-            if (pg) {
-                reinterpret_cast<uint4*>(pg)[v] = V::pack(gate + v * VEC);
-                reinterpret_cast<uint4*>(pu)[v] = V::pack(up + v * VEC);
-            }
+            for (int k = 0; k < 32 / VEC; ++k) reinterpret_cast<uint4*>(dst)[k] = V::pack(v + k * VEC);
+        } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) out[i] = gated_value<OutT>(t, gate[v * VEC + i], up[v * VEC + i], stays >> (v * VEC + i) & 1u);
-            reinterpret_cast<uint4*>(h)[v] = V::pack(out);
+            for (int i = 0; i < 32; ++i)  // fully unrolled: a dynamic index would push the accumulators to local memory
+                if (col0 + i < p.N) dst[i] = epi_from_float<OutT>(v[i]);
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {  // fully unrolled: a dynamic index would push the accumulators to local memory
-            if (col0 + i < p.N) {
-                if (pg) {
-                    pg[i] = epi_from_float<OutT>(gate[i]);
-                    pu[i] = epi_from_float<OutT>(up[i]);
-                }
-                h[i] = epi_from_float<OutT>(gated_value<OutT>(t, gate[i], up[i], stays >> i & 1u));
-            }
-        }
+    };
+    if (pg) {
+        store(pg, gate);
+        store(pu, up);
     }
+    gated_values<OutT>(t, static_cast<unsigned long long>(off), gate, up);
+    store(h, gate);
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
