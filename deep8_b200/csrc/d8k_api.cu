@@ -578,8 +578,9 @@ int d8k_ctx_create(int device, size_t scratch_bytes, d8k_ctx** out) {
     ctx->num_sms = prop.multiProcessorCount;
     ctx->scratch_bytes = scratch_bytes ? scratch_bytes : (static_cast<size_t>(64) << 20);
     cudaError_t e = cudaMalloc(&ctx->scratch, ctx->scratch_bytes);
-    if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, (kMaxCounters + 1) * sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, (kMaxCounters + 1) * sizeof(int));
+    // tickets, arrival words and the status word
+    if (e == cudaSuccess) e = cudaMalloc(&ctx->counters, (2 * kMaxCounters + 1) * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(ctx->counters, 0, (2 * kMaxCounters + 1) * sizeof(int));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->group_buf, sizeof(GroupEntry) * kMaxGroups);
     if (e != cudaSuccess) {
         cudaFree(ctx->scratch);
@@ -588,7 +589,8 @@ int d8k_ctx_create(int device, size_t scratch_bytes, d8k_ctx** out) {
         delete ctx;
         return fail(D8K_ERR_CUDA, std::string("d8k_ctx_create: ") + cudaGetErrorString(e));
     }
-    ctx->status = ctx->counters + kMaxCounters;
+    ctx->arrivals = reinterpret_cast<unsigned*>(ctx->counters + kMaxCounters);
+    ctx->status = ctx->counters + 2 * kMaxCounters;
     *out = ctx;
     return 0;
 }

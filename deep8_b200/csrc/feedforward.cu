@@ -6,7 +6,9 @@
 #include <cmath>
 #include <cstdint>
 #include <exception>
+#include <mutex>
 #include <string>
+#include <vector>
 
 #include "../../include/d8k.h"
 #include "elementwise.cuh"
@@ -27,7 +29,7 @@ namespace {
 // ------------------------------------------------------------------------------------------------ gated projections
 // A pack of W consecutive elements as one memory access: 16 bytes, or a single element where rows or bases are not aligned to that.
 template <typename T, int W>
-struct alignas(W * sizeof(T)) Pack {
+struct alignas(W * sizeof(T) < 16 ? W * sizeof(T) : 16) Pack {
     T v[W];
 };
 template <typename T, int W>
@@ -39,28 +41,207 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, W>& v) {
     *reinterpret_cast<Pack<T, W>*>(p) = v;
 }
 
+// True in every thread of the CTA that is the last of `total` to arrive at `word` (Ctx::arrivals); all that the CTAs wrote before is then
+// visible to it.  One atomic each, and the word is back at zero after the last: these kernels wait for nothing, so none of them can leave a
+// word half-way.  (The contractions' compare-and-swap tickets, drawn by 16 CTAs at once, cost as much as a small product.)
+__device__ __forceinline__ bool last_arrival(unsigned* word, unsigned total) {
+    __shared__ int last;
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicInc(word, total - 1) == total - 1;
+    __syncthreads();
+    __threadfence();
+    return last;
+}
+
+__device__ __forceinline__ uint4 load_stream(const void* p) {  // read once: not kept in L1
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+// The gated product for R rows of x at most (a token, or a few, while a model answers): bound by reading both weight matrices once, so
+// no tensor cores.  A CTA takes a strip of 16 packs of columns (of 16 bytes) and a slice of the contraction; its 16 groups of 16 threads
+// take every 16th k, each thread a pack of both projections, R products each in fp32.  The groups' sums meet in shared memory, the slices'
+// in scratch memory: the CTA that finishes a strip last adds them in slice order and forms h.
+template <typename T, int R>
+__global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T* __restrict__ x, const T* __restrict__ w, T* __restrict__ h, int rows_all, int cols,
+                                                         int width, int k_per_slice, float* __restrict__ partial, unsigned* arrivals, GatedTail tail) {
+    constexpr int V = 16 / sizeof(T), STRIP = 16 * V;
+    constexpr int CHUNK = R > 4 ? 256 : 512;  // k staged at a time
+    __shared__ alignas(16) float xs[CHUNK][R];
+    __shared__ float sums[8][2 * R * V][16];
+    const int lane = threadIdx.x & 15, kl = threadIdx.x >> 4;
+    const int c = blockIdx.x * STRIP + lane * V;
+    const int row0 = blockIdx.z * R, rows = min(rows_all - row0, R);  // this group of rows
+    x += static_cast<size_t>(row0) * cols;
+    arrivals += static_cast<size_t>(blockIdx.z) * gridDim.x;
+    partial += static_cast<size_t>(blockIdx.z) * gridDim.x * gridDim.y * (2 * R * STRIP);
+    const int k_begin = blockIdx.y * k_per_slice, k_end = min(cols, k_begin + k_per_slice);
+    const size_t second = static_cast<size_t>(cols) * width;
+    float g[R][V] = {}, u[R][V] = {};
+    for (int k0 = k_begin; k0 < k_end; k0 += CHUNK) {
+        const int count = min(CHUNK, k_end - k0);
+        __syncthreads();
+        for (int i = threadIdx.x; i < R * CHUNK; i += 256) {
+            const int r = i / CHUNK, k = i % CHUNK;
+            xs[k][r] = r < rows && k < count ? widen(x[static_cast<size_t>(r) * cols + k0 + k]) : 0.0f;
+        }
+        __syncthreads();
+        if (c < width) {
+            const T* wp = w + static_cast<size_t>(k0) * width + c;
+            constexpr int U = R > 4 ? 2 : 4;  // k per step: 2 U loads in flight
+            for (int k0u = kl; k0u < count; k0u += 16 * U) {
+                uint4 gv[U], uv[U];
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    const int k = k0u + 16 * q;
+                    gv[q] = uv[q] = make_uint4(0u, 0u, 0u, 0u);
+                    if (k < count) {
+                        gv[q] = load_stream(wp + static_cast<size_t>(k) * width);
+                        uv[q] = load_stream(wp + second + static_cast<size_t>(k) * width);
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < U; ++q) {
+                    const T* ge = reinterpret_cast<const T*>(&gv[q]);
+                    const T* ue = reinterpret_cast<const T*>(&uv[q]);
+                    // k is below CHUNK, a multiple of 16 U; from `count` on both factors are zeros
+                    const Pack<float, R> a_row = *reinterpret_cast<const Pack<float, R>*>(xs[k0u + 16 * q]);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float a = a_row.v[r];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            g[r][j] = fmaf(a, widen(ge[j]), g[r][j]);
+                            u[r][j] = fmaf(a, widen(ue[j]), u[r][j]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            g[r][j] += __shfl_xor_sync(0xffffffffu, g[r][j], 16);
+            u[r][j] += __shfl_xor_sync(0xffffffffu, u[r][j], 16);
+            if ((threadIdx.x & 16) == 0) {
+                sums[threadIdx.x >> 5][(2 * r) * V + j][lane] = g[r][j];
+                sums[threadIdx.x >> 5][(2 * r + 1) * V + j][lane] = u[r][j];
+            }
+        }
+    __syncthreads();
+    const int slices = gridDim.y;
+    float* mine = partial + (static_cast<size_t>(blockIdx.x) * slices + blockIdx.y) * (2 * R * STRIP);
+    // output i of the strip: row i / STRIP, column i % STRIP; the gate's sum and, R * STRIP further, the up projection's
+    auto summed = [&](int i, int which) {
+        const int r = i / STRIP, col = i % STRIP;
+        float t = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += sums[k][(2 * r + which) * V + col % V][col / V];
+        return t;
+    };
+    if (slices > 1) {
+        for (int i = threadIdx.x; i < R * STRIP; i += 256) {
+            __stcg(mine + i, summed(i, 0));
+            __stcg(mine + R * STRIP + i, summed(i, 1));
+        }
+        if (!last_arrival(arrivals + blockIdx.x, slices)) return;
+    }
+    const unsigned long long offset = tail.dropping ? drop_offset(tail.drop) : 0;
+    const float* first = partial + static_cast<size_t>(blockIdx.x) * slices * (2 * R * STRIP);
+    for (int i = threadIdx.x; i < R * STRIP; i += 256) {
+        const int r = i / STRIP, col = blockIdx.x * STRIP + i % STRIP;
+        if (r >= rows || col >= width) continue;
+        float gate, up;
+        if (slices > 1) {
+            gate = up = 0.0f;
+#pragma unroll 8
+            for (int s = 0; s < slices; ++s) {
+                gate += __ldcg(first + static_cast<size_t>(s) * (2 * R * STRIP) + i);
+                up += __ldcg(first + static_cast<size_t>(s) * (2 * R * STRIP) + R * STRIP + i);
+            }
+        } else {
+            gate = summed(i, 0);
+            up = summed(i, 1);
+        }
+        const size_t at = static_cast<size_t>(row0 + r) * width + col;
+        if (tail.pre) {
+            static_cast<T*>(tail.pre)[at] = narrow<T>(gate);
+            static_cast<T*>(tail.pre)[tail.pre_stride + at] = narrow<T>(up);
+        }
+        float out = 0.0f;
+        with_activation(tail.act, [&](auto which) {
+            float value, slope;
+            activation<decltype(which)::value, sizeof(T) == 2, false>(gate, value, slope);
+            out = value * up;
+        });
+        if (tail.dropping) {
+            const uint4 words = philox4x32(at >> 2, offset, tail.drop.seed);
+            const uint32_t word = (at & 3) == 0 ? words.x : (at & 3) == 1 ? words.y : (at & 3) == 2 ? words.z : words.w;
+            out = drop_keeps(tail.drop, word) ? out * tail.drop.scale : 0.0f;
+        }
+        h[at] = narrow<T>(out);
+    }
+}
+
+// widened elements of a pack and back; two halves per conversion where there are two
+template <typename T, int W>
+__device__ __forceinline__ void unpack(const Pack<T, W>& p, float (&f)[W]) {
+    if constexpr (sizeof(T) == 2 && W % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < W; k += 2) {
+            const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&p.v[k]));
+            f[k] = t.x;
+            f[k + 1] = t.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < W; ++k) f[k] = widen(p.v[k]);
+    }
+}
+template <typename T, int W>
+__device__ __forceinline__ Pack<T, W> pack_of(const float (&f)[W]) {
+    Pack<T, W> p;
+    if constexpr (sizeof(T) == 2 && W % 2 == 0) {
+#pragma unroll
+        for (int k = 0; k < W; k += 2) *reinterpret_cast<__half2*>(&p.v[k]) = __floats2half2_rn(f[k], f[k + 1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < W; ++k) p.v[k] = narrow<T>(f[k]);
+    }
+    return p;
+}
+
 // dpre from pre and dz: five accesses per element, bound by HBM (8192 x 16384 fp16: 234 us, 5.7 TB/s).  pre and dpre may be the same
 // memory (an element is read and written by one thread), so nothing here is declared __restrict__.
 template <int ACT, typename T, int E>
 __device__ __forceinline__ void gated_grad_elements(Pack<T, E>& g, Pack<T, E>& u, const Pack<T, E>& d, size_t i0, unsigned long long offset, const DropSpec& drop,
                                                     int dropping) {
     constexpr bool FAST = sizeof(T) == 2;
+    float gate[E], up[E], dd[E];
+    unpack(g, gate);
+    unpack(u, up);
+    unpack(d, dd);
 #pragma unroll
     for (int q = 0; q < E / 4; ++q) {
         uint4 words = make_uint4(0u, 0u, 0u, 0u);
         if (dropping) words = philox4x32((i0 >> 2) + q, offset, drop.seed);
         const uint32_t word[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 4 * q; k < 4 * q + 4; ++k) {
             float value, slope;
-            activation<ACT, FAST, true>(widen(g.v[4 * q + k]), value, slope);
-            const float dd = dropping ? widen(d.v[4 * q + k]) * drop.scale : widen(d.v[4 * q + k]);
-            float dg = dd * widen(u.v[4 * q + k]) * slope, du = dd * value;
-            if (dropping && !drop_keeps(drop, word[k])) dg = du = 0.0f;  // whatever the projections held
-            g.v[4 * q + k] = narrow<T>(dg);
-            u.v[4 * q + k] = narrow<T>(du);
+            activation<ACT, FAST, true>(gate[k], value, slope);
+            if (dropping) dd[k] *= drop.scale;
+            gate[k] = dd[k] * up[k] * slope;
+            up[k] = dd[k] * value;
+            if (dropping && !drop_keeps(drop, word[k - 4 * q])) gate[k] = up[k] = 0.0f;  // whatever the projections held
         }
     }
+    g = pack_of<T, E>(gate);
+    u = pack_of<T, E>(up);
 }
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const T* dz, T* dpre, size_t n, int act, DropSpec drop, int dropping) {
@@ -101,49 +282,39 @@ __global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const
 }
 
 // ------------------------------------------------------------------------------------------------ dropout
-// One pack of y = (residual +) dropout(x), i0 the index of its first element (a multiple of four)
+// One pack of y = (residual +) dropout(x); group: low word of the first four elements' counter
 template <typename T, int E>
-__device__ __forceinline__ void drop_pack(Pack<T, E>& a, const Pack<T, E>& b, bool add, size_t i0, unsigned long long offset, const DropSpec& drop) {
+__device__ __forceinline__ Pack<T, E> drop_pack(const Pack<T, E>& a, const Pack<T, E>& b, bool add, uint32_t group, uint32_t group_hi,
+                                                unsigned long long offset, const DropSpec& drop) {
+    float v[E], r[E];
+    unpack(a, v);
+    if (add) unpack(b, r);
 #pragma unroll
     for (int q = 0; q < E / 4; ++q) {
-        const uint4 words = philox4x32((i0 >> 2) + q, offset, drop.seed);
+        const uint4 words = philox4x32(group + q, group_hi, offset, drop.seed);
         const uint32_t word[4] = {words.x, words.y, words.z, words.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            float v = drop_keeps(drop, word[k]) ? widen(a.v[4 * q + k]) * drop.scale : 0.0f;
-            if (add) v += widen(b.v[4 * q + k]);
-            a.v[4 * q + k] = narrow<T>(v);
+        for (int k = 4 * q; k < 4 * q + 4; ++k) {
+            v[k] = drop_keeps(drop, word[k - 4 * q]) ? v[k] * drop.scale : 0.0f;
+            if (add) v[k] += r[k];
         }
     }
+    return pack_of<T, E>(v);
 }
 // y = (residual +) dropout(x): `residual` is the accumulated gradient itself in the backward pass.  VEC: bases on 16-byte boundaries; the
-// last, partial pack goes element by element either way.  y may be x or residual, so nothing is declared __restrict__.
+// last, partial pack goes element by element either way.  A launch covers at most 2^34 elements, whose counters share their high
+// word.  y may be x or residual, so nothing is declared __restrict__.
 template <typename T, bool VEC, bool ADD>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, T* y, size_t n, DropSpec drop) {
+__global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, T* y, size_t n, uint32_t group_hi, DropSpec drop) {
     constexpr int E = VEC ? 16 / sizeof(T) : 4;
     const unsigned long long offset = drop_offset(drop);
     const size_t whole = n / E, stride = gridDim.x * static_cast<size_t>(blockDim.x);
     size_t s = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x;
     if (VEC) {
-        constexpr int U = 2;  // packs in flight per thread
-        for (; s + (U - 1) * stride < whole; s += U * stride) {
-            Pack<T, E> a[U], b[U] = {};
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                a[k] = load_pack<T, E>(x + (s + k * stride) * E);
-                if (ADD) b[k] = load_pack<T, E>(residual + (s + k * stride) * E);
-            }
-#pragma unroll
-            for (int k = 0; k < U; ++k) {
-                drop_pack(a[k], b[k], ADD, (s + k * stride) * E, offset, drop);
-                store_pack(y + (s + k * stride) * E, a[k]);
-            }
-        }
         for (; s < whole; s += stride) {
             Pack<T, E> a = load_pack<T, E>(x + s * E), b = {};
             if (ADD) b = load_pack<T, E>(residual + s * E);
-            drop_pack(a, b, ADD, s * E, offset, drop);
-            store_pack(y + s * E, a);
+            store_pack(y + s * E, drop_pack(a, b, ADD, static_cast<uint32_t>(s * (E / 4)), group_hi, offset, drop));
         }
     }
     for (; s * E < n; s += stride) {
@@ -154,7 +325,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* resid
                 a.v[k] = x[s * E + k];
                 if (ADD) b.v[k] = residual[s * E + k];
             }
-        drop_pack(a, b, ADD, s * E, offset, drop);
+        a = drop_pack(a, b, ADD, static_cast<uint32_t>(s * (E / 4)), group_hi, offset, drop);
 #pragma unroll
         for (int k = 0; k < E; ++k)
             if (s * E + k < n) y[s * E + k] = a.v[k];
@@ -199,9 +370,12 @@ __global__ void __launch_bounds__(512) rms_norm_forward_kernel(const T* x, const
             if (live && i < packs) v[k] = load_pack<T, W>(row + static_cast<size_t>(i) * W);
         }
 #pragma unroll
-        for (int k = 0; k < N; ++k)
+        for (int k = 0; k < N; ++k) {
+            float f[W];
+            unpack(v[k], f);
 #pragma unroll
-            for (int j = 0; j < W; ++j) sum = fmaf(widen(v[k].v[j]), widen(v[k].v[j]), sum);
+            for (int j = 0; j < W; ++j) sum = fmaf(f[j], f[j], sum);
+        }
         sum = row_sum(sum, tpr, part[buf]);
         const float inv = 1.0f / sqrtf(sum / cols + eps);
         if (live && rstd && at == 0) rstd[r] = inv;
@@ -209,10 +383,12 @@ __global__ void __launch_bounds__(512) rms_norm_forward_kernel(const T* x, const
         for (int k = 0; k < N; ++k) {
             const int i = at + k * tpr;
             if (live && i < packs) {
-                const Pack<T, W> w = load_pack<T, W>(weight + static_cast<size_t>(i) * W);
+                float f[W], w[W];
+                unpack(v[k], f);
+                unpack(load_pack<T, W>(weight + static_cast<size_t>(i) * W), w);
 #pragma unroll
-                for (int j = 0; j < W; ++j) v[k].v[j] = narrow<T>(widen(v[k].v[j]) * inv * widen(w.v[j]));
-                store_pack(y + r * cols + static_cast<size_t>(i) * W, v[k]);
+                for (int j = 0; j < W; ++j) f[j] *= inv * w[j];
+                store_pack(y + r * cols + static_cast<size_t>(i) * W, pack_of<T, W>(f));
             }
         }
     }
@@ -235,10 +411,10 @@ __global__ void __launch_bounds__(512) rms_norm_backward_kernel(const T* __restr
 #pragma unroll
         for (int j = 0; j < W; ++j) dw[k][j] = 0.0f;
     Pack<T, W> xs[N], gs[N];
-    float inv = 0.0f;
+    float next_inv = 0.0f;
     auto fetch = [&](size_t r) {
         const bool live = r < rows;
-        inv = live ? rstd[r] : 0.0f;
+        next_inv = live ? rstd[r] : 0.0f;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int i = at + k * tpr;
@@ -253,19 +429,22 @@ __global__ void __launch_bounds__(512) rms_norm_backward_kernel(const T* __restr
     int buf = 0;
     for (size_t r0 = blockIdx.x * static_cast<size_t>(group); r0 < rows; r0 += step, buf ^= 1) {
         const size_t r = r0 + sub;
-        const float scale = inv;
+        const float inv = next_inv;
         float n[N][W], u[N][W], sum = 0.0f;  // x * rstd, dy * weight
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int i = at + k * tpr;
-            Pack<T, W> w = {};
-            if (i < packs) w = load_pack<T, W>(weight + static_cast<size_t>(i) * W);
+            float w[W];
+            Pack<T, W> wp = {};
+            if (i < packs) wp = load_pack<T, W>(weight + static_cast<size_t>(i) * W);
+            unpack(wp, w);
+            unpack(xs[k], n[k]);
+            unpack(gs[k], u[k]);
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const float g = widen(gs[k].v[j]);
-                n[k][j] = widen(xs[k].v[j]) * scale;
-                u[k][j] = g * widen(w.v[j]);
-                dw[k][j] = fmaf(g, n[k][j], dw[k][j]);
+                n[k][j] *= inv;
+                dw[k][j] = fmaf(u[k][j], n[k][j], dw[k][j]);
+                u[k][j] *= w[j];
                 sum = fmaf(u[k][j], n[k][j], sum);
             }
         }
@@ -275,14 +454,13 @@ __global__ void __launch_bounds__(512) rms_norm_backward_kernel(const T* __restr
 #pragma unroll
         for (int k = 0; k < N; ++k) {
             const int i = at + k * tpr;
-            if (r < rows && i < packs) {
-                T* dst = dx + r * cols + static_cast<size_t>(i) * W;
-                Pack<T, W> out = {};
-                if (accumulate) out = load_pack<T, W>(dst);
+            if (r >= rows || i >= packs) continue;
+            T* dst = dx + r * cols + static_cast<size_t>(i) * W;
+            float out[W] = {};
+            if (accumulate) unpack(load_pack<T, W>(dst), out);
 #pragma unroll
-                for (int j = 0; j < W; ++j) out.v[j] = narrow<T>(fmaf(scale, u[k][j] - n[k][j] * mean, accumulate ? widen(out.v[j]) : 0.0f));
-                store_pack(dst, out);
-            }
+            for (int j = 0; j < W; ++j) out[j] = fmaf(inv, fmaf(-n[k][j], mean, u[k][j]), out[j]);
+            store_pack(dst, pack_of<T, W>(out));
         }
     }
     if (!partial) return;
@@ -435,11 +613,33 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 }
 size_t esize(int dtype) { return dtype == D8K_F32 ? 4 : 2; }
 
-int grid_for(const d8k_ctx* ctx, size_t steps) {
-    size_t blocks = (steps + 255) / 256;
-    const size_t cap = static_cast<size_t>(ctx->num_sms) * 8;
-    if (blocks > cap) blocks = cap;
-    return blocks < 1 ? 1 : static_cast<int>(blocks);
+// CTAs of `kernel` that one SM holds at once.  Asked once per kernel, block size and shared memory and kept: the driver's answer costs as
+// much as a launch.
+template <class Kernel>
+int resident_ctas(Kernel* kernel, int threads, size_t dyn = 0) {
+    struct Entry {
+        const void* kernel;
+        int threads;
+        size_t dyn;
+        int ctas;
+    };
+    static std::mutex mutex;
+    static std::vector<Entry> known;
+    std::lock_guard<std::mutex> lock(mutex);
+    for (const Entry& e : known)
+        if (e.kernel == reinterpret_cast<const void*>(kernel) && e.threads == threads && e.dyn == dyn) return e.ctas;
+    int ctas = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, threads, dyn) != cudaSuccess || ctas < 1) ctas = 1;
+    if (known.size() < 256) known.push_back(Entry{reinterpret_cast<const void*>(kernel), threads, dyn, ctas});
+    return ctas;
+}
+
+// A grid for `steps` steps of one thread each, all of whose CTAs are in work at once: with a fixed eight per SM a kernel of which five fit
+// ran a second, emptier round (dropout 49 us for 37).
+template <class Kernel>
+unsigned grid_for(const d8k_ctx* ctx, Kernel* kernel, size_t steps) {
+    const size_t blocks = (steps + 255) / 256, cap = static_cast<size_t>(ctx->num_sms) * resident_ctas(kernel, 256);
+    return static_cast<unsigned>(blocks > cap ? cap : blocks < 1 ? 1 : blocks);
 }
 
 // The launch's form of a dropout argument; *on stays 0 when there is nothing to drop (none given, or p == 0).
@@ -465,6 +665,29 @@ int check_gated(int activation, int xb, int xr, int xc, int yc) {
     if (xb < 0 || xr < 0 || xc < 1 || yc < 1) return fail(D8K_ERR_ARGUMENT, "the shape is error");
     if (1LL * xb * xr >= (1LL << 31)) return fail(D8K_ERR_ARGUMENT, "the shape is too large");
     return 0;
+}
+
+// The fp32 product for up to 16 rows in groups of one, two, four or eight, true when it is this kernel's: whole 16-byte packs of columns at
+// 16-byte boundaries, and strips few enough for the arrival words.  (fp16 has gemm_gated_few.cu, which reads as fast for any of these row
+// counts.)  As many slices as are in work at once, of at least 64 k.
+bool gated_rows(d8k_ctx* ctx, const float* x, const float* w, float* h, int rows, int cols, int width, const GatedTail& tail) {
+    constexpr int V = 4;
+    const int strips = (width + 16 * V - 1) / (16 * V), groups = (rows + 7) / 8;
+    if (rows > 8 || width % V != 0 || !aligned16({w}) || strips * groups > kMaxCounters) return false;
+    const int r = rows <= 2 ? rows : rows <= 4 ? 4 : 8;
+    auto kernel = r == 1 ? gated_rows_kernel<float, 1> : r == 2 ? gated_rows_kernel<float, 2> : r == 4 ? gated_rows_kernel<float, 4> : gated_rows_kernel<float, 8>;
+    long long slices = static_cast<long long>(ctx->num_sms) * resident_ctas(kernel, 256) / (strips * groups);
+    if (slices > cols / 64) slices = cols / 64;
+    const long long most = static_cast<long long>(ctx->scratch_bytes / (static_cast<size_t>(strips) * groups * 2 * r * 16 * V * sizeof(float)));
+    if (slices > most) slices = most;
+    if (slices > 255) slices = 255;
+    if (slices < 1) slices = 1;
+    int per = static_cast<int>((cols + slices - 1) / slices);
+    per = (per + 15) / 16 * 16;
+    slices = (cols + per - 1) / per;
+    kernel<<<dim3(strips, static_cast<unsigned>(slices), groups), 256, 0, ctx->stream>>>(x, w, h, rows, cols, width, per, ctx->scratch,
+                                                                               ctx->arrivals, tail);
+    return true;
 }
 
 int check_norm(size_t rows, int cols) {
@@ -495,11 +718,10 @@ int gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, con
         return fail(D8K_ERR_ARGUMENT, "gated: dpre overlaps an input");
     const int per = static_cast<int>(16 / esize(dtype));
     const bool vec = aligned16({pre, dz, dpre}) && n % per == 0;
-    const int grid = grid_for(ctx, (n + per - 1) / (vec ? per : 4));
     auto run = [&](auto zero) {
         using T = decltype(zero);
         auto kernel = vec ? gated_grad_pre_kernel<T, true> : gated_grad_pre_kernel<T, false>;
-        kernel<<<grid, 256, 0, ctx->stream>>>(static_cast<const T*>(pre), static_cast<const T*>(dz), static_cast<T*>(dpre), n, activation, spec, dropping);
+        kernel<<<grid_for(ctx, kernel, (n + per - 1) / (vec ? per : 4)), 256, 0, ctx->stream>>>(static_cast<const T*>(pre), static_cast<const T*>(dz), static_cast<T*>(dpre), n, activation, spec, dropping);
     };
     if (dtype == D8K_F32) run(0.0f);
     else run(__half());
@@ -562,17 +784,22 @@ int dropout(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* 
         return fail(D8K_ERR_ARGUMENT, "dropout: the output overlaps an input");
     const int per = static_cast<int>(16 / esize(dtype));
     const bool vec = aligned16({x, residual, y});
-    const int grid = grid_for(ctx, (n + per - 1) / (vec ? per : 4));
     auto run = [&](auto zero) {
         using T = decltype(zero);
         auto kernel = residual ? (vec ? dropout_kernel<T, true, true> : dropout_kernel<T, false, true>)
                                : (vec ? dropout_kernel<T, true, false> : dropout_kernel<T, false, false>);
-        kernel<<<grid, 256, 0, ctx->stream>>>(static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<T*>(y), n, spec);
+        constexpr size_t kMost = static_cast<size_t>(1) << 34;  // elements whose counters share their high word
+        for (size_t first = 0; first < n; first += kMost) {
+            const size_t count = n - first < kMost ? n - first : kMost;
+            kernel<<<grid_for(ctx, kernel, (count + per - 1) / (vec ? per : 4)), 256, 0, ctx->stream>>>(
+                static_cast<const T*>(x) + first, residual ? static_cast<const T*>(residual) + first : nullptr, static_cast<T*>(y) + first, count,
+                static_cast<uint32_t>(first >> 34), spec);
+            count_launch();
+        }
     };
     if (dtype == D8K_F32) run(0.0f);
     else run(__half());
     D8K_CUDA(cudaGetLastError());
-    count_launch();
     return 0;
 }
 
@@ -582,12 +809,12 @@ int dropout(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* 
 struct RowPlan {
     int tpr, packs_per_thread, threads, group;
 };
-RowPlan plan_rows(const d8k_ctx* ctx, size_t rows, int packs, bool vec, int start) {
+RowPlan plan_rows(const d8k_ctx* ctx, size_t rows, int packs, bool vec, int start, int least_threads) {
     for (int n = rows < static_cast<size_t>(ctx->num_sms) * 4 ? 1 : start; n <= (vec ? 4 : 16); n *= vec ? 2 : 4) {
         int tpr = 32;
         while (tpr < 512 && static_cast<long long>(tpr) * n < packs) tpr *= 2;
         if (static_cast<long long>(tpr) * n < packs) continue;
-        const int threads = tpr > 256 ? tpr : 256;
+        const int threads = tpr > least_threads ? tpr : least_threads;
         return RowPlan{tpr, n, threads, threads / tpr};
     }
     return RowPlan{0, 0, 0, 0};
@@ -597,16 +824,17 @@ template <typename T>
 int rms_norm_forward(d8k_ctx* ctx, const T* x, const T* weight, float eps, T* y, float* rstd, size_t rows, int cols) {
     constexpr int W = 16 / sizeof(T);
     const bool vec = aligned16({x, weight, y}) && cols % W == 0;
-    const RowPlan p = plan_rows(ctx, rows, vec ? cols / W : cols, vec, 4);
+    const RowPlan p = plan_rows(ctx, rows, vec ? cols / W : cols, vec, 4, 256);
     if (p.packs_per_thread == 0) {
         const size_t cap = static_cast<size_t>(ctx->num_sms) * 4;
         rms_norm_forward_long_kernel<T><<<static_cast<unsigned>(rows < cap ? rows : cap), 512, 0, ctx->stream>>>(x, weight, y, rstd, rows, cols, eps);
     } else {
-        const size_t groups = (rows + p.group - 1) / p.group, cap = static_cast<size_t>(ctx->num_sms) * (2048 / p.threads);
+        const size_t groups = (rows + p.group - 1) / p.group;
         auto kernel = vec ? (p.packs_per_thread == 1 ? rms_norm_forward_kernel<T, W, 1> : p.packs_per_thread == 2 ? rms_norm_forward_kernel<T, W, 2>
                                                                                                             : rms_norm_forward_kernel<T, W, 4>)
                           : (p.packs_per_thread == 1 ? rms_norm_forward_kernel<T, 1, 1> : p.packs_per_thread == 4 ? rms_norm_forward_kernel<T, 1, 4>
                                                                                                             : rms_norm_forward_kernel<T, 1, 16>);
+        const size_t cap = static_cast<size_t>(ctx->num_sms) * resident_ctas(kernel, p.threads);
         kernel<<<static_cast<unsigned>(groups < cap ? groups : cap), p.threads, 0, ctx->stream>>>(x, weight, y, rstd, rows, cols, eps, p.tpr);
     }
     D8K_CUDA(cudaGetLastError());
@@ -618,7 +846,7 @@ template <typename T>
 int rms_norm_backward(d8k_ctx* ctx, const T* x, const T* weight, const float* rstd, T* dx, T* dweight, const T* dy, size_t rows, int cols, int accumulate) {
     constexpr int W = 16 / sizeof(T);
     const bool vec = aligned16({x, weight, dx, dy}) && cols % W == 0;
-    const RowPlan p = plan_rows(ctx, rows, vec ? cols / W : cols, vec, vec ? 2 : 4);
+    const RowPlan p = plan_rows(ctx, rows, vec ? cols / W : cols, vec, vec ? 2 : 4, 512);
     const size_t most = ctx->scratch_bytes / (static_cast<size_t>(cols) * sizeof(float));  // slices of column sums the scratch memory holds
     if (dweight && most < 1) return fail(D8K_ERR_ARGUMENT, "the context's scratch memory is smaller than one row of floats");
     if (!dx && !dweight) return 0;
@@ -630,9 +858,7 @@ int rms_norm_backward(d8k_ctx* ctx, const T* x, const T* weight, const float* rs
                           : (p.packs_per_thread == 1 ? rms_norm_backward_kernel<T, 1, 1> : p.packs_per_thread == 4 ? rms_norm_backward_kernel<T, 1, 4>
                                                                                                              : rms_norm_backward_kernel<T, 1, 16>);
         const size_t dyn = dweight ? static_cast<size_t>(p.group - 1) * cols * sizeof(float) : 0;
-        int per_sm = 0;
-        D8K_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, p.threads, dyn));
-        slices = static_cast<size_t>(ctx->num_sms) * (per_sm < 1 ? 1 : per_sm);
+        slices = static_cast<size_t>(ctx->num_sms) * resident_ctas(kernel, p.threads, dyn);
         if (slices > groups) slices = groups;
         if (dweight && slices > most) slices = most;
         kernel<<<static_cast<unsigned>(slices), p.threads, dyn, ctx->stream>>>(x, weight, rstd, dx, dweight ? ctx->scratch : nullptr, dy, rows, cols, accumulate,
@@ -686,13 +912,20 @@ int d8k_gated_forward(d8k_ctx* ctx, int dtype, int activation, const void* x, in
         const size_t es = esize(dtype), xs = es * rows * xc, ws = 2 * es * xc * yc, hs = es * rows * yc;
         if (overlap(h, hs, x, xs) || overlap(h, hs, w, ws) || overlap(pre, 2 * hs, x, xs) || overlap(pre, 2 * hs, w, ws) || overlap(pre, 2 * hs, h, hs))
             return fail(D8K_ERR_ARGUMENT, "gated: an output overlaps an input or the other output");
+        const GatedTail tail{activation, dropping, pre, 1LL * rows * yc, spec};
+        if (dtype == D8K_F32 && gated_rows(ctx, static_cast<const float*>(x), static_cast<const float*>(w), static_cast<float*>(h), rows, xc, yc, tail)) {
+            D8K_CUDA(cudaGetLastError());
+            count_launch();
+            set_last_kernel("f32 gated rows");
+            return 0;
+        }
         GatedProblem g;
         g.dtype = dtype;
         g.M = rows; g.N = yc; g.K = xc;
         g.a = x;
         g.b = w;
         g.C = h;
-        g.tail = GatedTail{activation, dropping, pre, 1LL * rows * yc, spec};
+        g.tail = tail;
         return run_gated(ctx, g);
     });
 }

@@ -18,6 +18,7 @@ struct Ctx {
     size_t scratch_bytes = 0;
     int* counters = nullptr;   // kMaxCounters tile ticket words (GemmParams::counters)
     unsigned epoch_counter = 0;  // this context's split launches so far, modulo 2^24 (GemmParams::epoch)
+    unsigned* arrivals = nullptr;  // kMaxCounters words, zero between launches: kernels whose last CTA finishes the work count their CTAs here
     int* status = nullptr;     // device status word
     GroupEntry* group_buf = nullptr;  // device memory for kMaxGroups entries of a grouped launch (null: launches are never grouped)
 };
@@ -79,6 +80,19 @@ struct GatedProblem {
     void* C = nullptr;
     GatedTail tail = {};
 };
+
+// the kernel for a few rows (gemm_gated_few.cu)
+struct GatedFewParams {
+    int rows, width;
+    int num_kb, splits, kb_per_split;  // in stages of 64 k, or 128 for up to 32 tokens
+    int total_work;                    // strips of 128 columns x splits; split launches have one CTA per item, a cluster per strip
+    int x_chunked, w_chunked;
+    int* status;
+    void* h;
+    GatedTail gated;
+};
+// tokens: 16, 32, 64 or 128, at least the rows
+cudaError_t launch_gated_few(int tokens, int grid, cudaStream_t stream, const CUtensorMap& tx, const CUtensorMap& tw, const GatedFewParams& p);
 
 // error reporting shared by the API layer
 void set_error(const std::string& msg);

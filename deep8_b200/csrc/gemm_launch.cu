@@ -652,6 +652,49 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
     return 0;
 }
 
+// The kernel for up to 128 rows of fp16 (gemm_gated_few.cu).
+static int run_gated_few(Ctx* ctx, const GatedProblem& g, const HostOperand& x, const HostOperand& w) {
+    GatedFewParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.rows = g.M;
+    p.width = g.N;
+    const int tokens = g.M <= 16 ? 16 : g.M <= 32 ? 32 : g.M <= 64 ? 64 : 128;
+    const int sub = tokens <= 32 ? 2 : 1;  // k-blocks of 64 per stage (FewCfg::SUB)
+    p.num_kb = (g.K + 64 * sub - 1) / (64 * sub);
+    const int strips = (g.N + 127) / 128;
+    // A CTA reads at most 94 GB/s, so few strips cannot use the memory's bandwidth: about 68 would.  Split until a CTA's share is what the
+    // memory needs for its part, but not below three double k-blocks, which the launch's fixed time hides (measured on 2048 -> 2 x 5504, 43 strips:
+    // 16.5 us unsplit, 13.0 with 2, 13.3 with 3, 19.7 with 4; 4096 -> 2 x 1024, 8 strips: 27.7 unsplit, 12.3 with 4, 11.0 with 8).  All clusters have
+    // to be in work at once: those of more than four CTAs leave SMs of a GPC unused (8 x 16 strips took two rounds).
+    long long share = static_cast<long long>(strips) * p.num_kb / 68;
+    if (share < 6 / sub) share = 6 / sub;
+    int splits = static_cast<int>((p.num_kb + share - 1) / share);
+    if (splits > 8) splits = 8;
+    while (splits > 1 && strips * splits > (splits > 4 ? 96 : 132)) --splits;
+    p.kb_per_split = (p.num_kb + splits - 1) / splits;
+    p.splits = (p.num_kb + p.kb_per_split - 1) / p.kb_per_split;
+    p.total_work = strips * p.splits;
+    p.x_chunked = g.K % 64 == 0;
+    p.w_chunked = g.N % 64 == 0;
+    p.status = ctx->status;
+    p.h = g.C;
+    p.gated = g.tail;
+    CUtensorMap tx, tw;
+    std::memset(&tx, 0, sizeof(tx));
+    std::memset(&tw, 0, sizeof(tw));
+    if (!(p.x_chunked ? make_pair_map(&tx, x, g.M, g.K, tokens, sub) : make_map(&tx, x, g.K, g.M, tokens)) ||
+        !(p.w_chunked ? make_pair_map(&tw, w, g.N, g.K, 64 * sub, 2) : make_map(&tw, w, g.N, g.K, 64 * sub)))
+        return fail(2, "gated: cuTensorMapEncodeTiled failed");
+    const int grid = p.splits > 1 || p.total_work < ctx->num_sms ? p.total_work : ctx->num_sms;
+    cudaError_t e = launch_gated_few(tokens, grid, ctx->stream, tx, tw, p);
+    if (e != cudaSuccess) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
+    count_launch();
+    std::ostringstream os;
+    os << "f16 gated few tokens=" << tokens << " splits=" << p.splits << " grid=" << grid;
+    set_last_kernel(os.str());
+    return 0;
+}
+
 int run_gated(Ctx* ctx, const GatedProblem& g) {
     const bool f32 = g.dtype == 1;
     const int esize = f32 ? 4 : 2, bk = 128 / esize;
@@ -664,6 +707,7 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     b.batch_count = 2;
     b.batch_stride = static_cast<long long>(g.K) * g.N;
     const bool tma = tma_ok(a, esize) && tma_ok(b, esize) && encode_tiled() != nullptr && !env_int("D8K_FORCE_GATHER", 0);
+    if (tma && !f32 && g.M <= 128) return run_gated_few(ctx, g, a, b);
     const long long mtiles = (g.M + kBM - 1) / kBM, ptiles = (g.M + 255LL) / 256 * ((g.N + 127) / 128);
     // The paired kernel from half a wave of its tiles on, with a long contraction from a third of one, as in make_plan.
     const bool pair = tma && !f32 && g.K % 64 == 0 && g.N % 64 == 0 && env_int("D8K_PAIR", 1) != 0 &&
