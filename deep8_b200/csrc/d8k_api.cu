@@ -601,6 +601,7 @@ int d8k_ctx_destroy(d8k_ctx* ctx) {
     cudaFree(ctx->scratch);
     cudaFree(ctx->counters);
     cudaFree(ctx->group_buf);
+    for (void* p : ctx->pads) cudaFree(p);
     delete ctx;
     return 0;
 }

@@ -215,6 +215,31 @@ __device__ __forceinline__ Pack<T, W> pack_of(const float (&f)[W]) {
     return p;
 }
 
+// Copies of row-major matrices with their rows padded by zeros to whole 128-byte pieces, so that TMA can read what starts anywhere:
+// one 16-byte store per step, its elements loaded one by one.
+struct PadJobs {
+    PadJob job[2];
+};
+template <typename T>
+__global__ void __launch_bounds__(256) pad_kernel(PadJobs jobs, int count) {
+    constexpr int W = 16 / sizeof(T);
+    for (int q = 0; q < count; ++q) {
+        const T* src = static_cast<const T*>(jobs.job[q].src);
+        T* dst = static_cast<T*>(jobs.job[q].dst);
+        const int cols = jobs.job[q].cols, packs = jobs.job[q].pitch / W;
+        const size_t total = static_cast<size_t>(jobs.job[q].rows) * packs;
+        for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
+            const size_t r = i / packs;
+            const int c = static_cast<int>(i - r * packs) * W;
+            const T* from = src + r * cols + c;
+            Pack<T, W> v;
+#pragma unroll
+            for (int k = 0; k < W; ++k) v.v[k] = c + k < cols ? from[k] : narrow<T>(0.0f);
+            store_pack(dst + i * W, v);
+        }
+    }
+}
+
 // dpre from pre and dz: five accesses per element, bound by HBM (8192 x 16384 fp16: 234 us, 5.7 TB/s).  pre and dpre may be the same
 // memory (an element is read and written by one thread), so nothing here is declared __restrict__.
 template <int ACT, typename T, int E>
@@ -244,10 +269,11 @@ __device__ __forceinline__ void gated_grad_elements(Pack<T, E>& g, Pack<T, E>& u
     u = pack_of<T, E>(up);
 }
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const T* dz, T* dpre, size_t n, int act, DropSpec drop, int dropping) {
+__global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const T* dz, T* dpre, size_t n, int act, DropSpec drop, int dropping,
+                                                             unsigned width, unsigned pitch) {
     constexpr int E = VEC ? 16 / sizeof(T) : 4;
     const unsigned long long offset = dropping ? drop_offset(drop) : 0;
-    const size_t steps = (n + E - 1) / E, stride = gridDim.x * static_cast<size_t>(blockDim.x);
+    const size_t steps = (n + E - 1) / E, stride = gridDim.x * static_cast<size_t>(blockDim.x), second = n / width * pitch;
     with_activation(act, [&](auto which) {
         for (size_t s = blockIdx.x * static_cast<size_t>(blockDim.x) + threadIdx.x; s < steps; s += stride) {
             const size_t i0 = s * E;
@@ -273,8 +299,9 @@ __global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const
 #pragma unroll
                 for (int k = 0; k < E; ++k)
                     if (i0 + k < n) {
-                        dpre[i0 + k] = g.v[k];
-                        dpre[n + i0 + k] = u.v[k];
+                        const size_t r = (i0 + k) / width, at = r * pitch + (i0 + k - r * width);  // rows of dpre may be padded
+                        dpre[at] = g.v[k];
+                        dpre[second + at] = u.v[k];
                     }
             }
         }
@@ -706,22 +733,26 @@ HostOperand matrix(const void* ptr, bool mn, long long ld, int batch = 1, long l
     return o;
 }
 
-int gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, const void* dz, void* dpre, size_t n, const d8k_dropout* drop) {
+// dpre's rows (of `width` elements, n in all) are written `pitch` apart
+int gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, const void* dz, void* dpre, size_t n, size_t width, size_t pitch,
+                   const d8k_dropout* drop) {
     if (activation < 0 || activation >= kActCount) return fail(D8K_ERR_ARGUMENT, "gated: no such activation");
     DropSpec spec;
     int dropping = 0;
     if (int rc = make_drop(drop, &spec, &dropping)) return rc;
     if (n == 0) return 0;
     if (!pre || !dz || !dpre) return fail(D8K_ERR_ARGUMENT, "gated: null pointer");
-    const size_t bytes = n * esize(dtype);
-    if ((dpre != pre && overlap(dpre, 2 * bytes, pre, 2 * bytes)) || overlap(dpre, 2 * bytes, dz, bytes))
+    const size_t bytes = n * esize(dtype), out_bytes = n / width * pitch * esize(dtype);
+    if (((dpre != pre || pitch != width) && overlap(dpre, 2 * out_bytes, pre, 2 * bytes)) || overlap(dpre, 2 * out_bytes, dz, bytes))
         return fail(D8K_ERR_ARGUMENT, "gated: dpre overlaps an input");
     const int per = static_cast<int>(16 / esize(dtype));
-    const bool vec = aligned16({pre, dz, dpre}) && n % per == 0;
+    const bool vec = aligned16({pre, dz, dpre}) && n % per == 0 && pitch == width;
     auto run = [&](auto zero) {
         using T = decltype(zero);
         auto kernel = vec ? gated_grad_pre_kernel<T, true> : gated_grad_pre_kernel<T, false>;
-        kernel<<<grid_for(ctx, kernel, (n + per - 1) / (vec ? per : 4)), 256, 0, ctx->stream>>>(static_cast<const T*>(pre), static_cast<const T*>(dz), static_cast<T*>(dpre), n, activation, spec, dropping);
+        kernel<<<grid_for(ctx, kernel, (n + per - 1) / (vec ? per : 4)), 256, 0, ctx->stream>>>(
+            static_cast<const T*>(pre), static_cast<const T*>(dz), static_cast<T*>(dpre), n, activation, spec, dropping, static_cast<unsigned>(width),
+            static_cast<unsigned>(pitch));
     };
     if (dtype == D8K_F32) run(0.0f);
     else run(__half());
@@ -730,45 +761,81 @@ int gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, con
     return 0;
 }
 
-int gated_grad_x(d8k_ctx* ctx, int dtype, void* dx, int xb, int xr, int xc, const void* w, int yc, const void* dpre, int accumulate) {
-    if (int rc = check_gated(0, xb, xr, xc, yc)) return rc;
-    const int rows = xb * xr;
-    if (rows == 0) return 0;
-    if (!dx || !w || !dpre) return fail(D8K_ERR_ARGUMENT, "gated: null pointer");
-    const size_t es = esize(dtype), x_bytes = es * rows * xc;
-    if (overlap(dx, x_bytes, w, 2 * es * xc * yc) || overlap(dx, x_bytes, dpre, 2 * es * rows * yc)) return fail(D8K_ERR_ARGUMENT, "gated: dx overlaps an input");
+// The operands of the two gradient products: x [rows, xc], w and dpre [2, ...].  Where their rows do not start on 16-byte boundaries the
+// products read copies with padded rows (in the context's padding memory) that TMA can describe; the loader warps would fetch such rows
+// element by element (333 x 250 x 1001 fp32: 203 us for both gradients).
+struct GatedOperands {
+    HostOperand x, w, dpre;
+};
+// dpre_to_come: dpre is not there yet (gated_backward writes it): its place is chosen, nothing copied.  x or w without a pointer is left out.
+int gated_operands(d8k_ctx* ctx, int dtype, GatedOperands* o, const void* x, const void* w, const void* dpre, int rows, int xc, int yc, bool dpre_to_come) {
+    o->x = matrix(x, true, xc);
+    o->w = matrix(w, false, yc, 2, 1LL * xc * yc);
+    o->dpre = matrix(dpre, false, yc, 2, 1LL * rows * yc);
+    const int piece = static_cast<int>(128 / esize(dtype));
+    struct Part {
+        HostOperand* o;
+        long long rows;
+        int cols;
+    } parts[3] = {{&o->x, rows, xc}, {&o->w, 2LL * xc, yc}, {&o->dpre, 2LL * rows, yc}};
+    size_t bytes = 0, at[3] = {};
+    bool wanted[3] = {};
+    for (int k = 0; k < 3; ++k) {
+        wanted[k] = parts[k].o->ptr && !rows_aligned(parts[k].o->ptr, parts[k].cols, dtype);
+        at[k] = bytes;
+        if (wanted[k]) bytes += (static_cast<size_t>(parts[k].rows) * ((parts[k].cols + piece - 1) / piece * piece) * esize(dtype) + 255) & ~static_cast<size_t>(255);
+    }
+    char* base = bytes ? static_cast<char*>(pad_memory(ctx, bytes)) : nullptr;
+    if (!base) return 0;
+    PadJob jobs[3];
+    int count = 0;
+    for (int k = 0; k < 3; ++k) {
+        if (!wanted[k]) continue;
+        HostOperand& h = *parts[k].o;
+        const int pitch = (parts[k].cols + piece - 1) / piece * piece;
+        if (k != 2 || !dpre_to_come) {
+            jobs[count].src = h.ptr;
+            jobs[count].dst = base + at[k];
+            jobs[count].rows = parts[k].rows;
+            jobs[count].cols = parts[k].cols;
+            jobs[count++].pitch = pitch;
+        }
+        h.ptr = base + at[k];
+        h.ld = pitch;
+        h.padded = true;
+        if (h.batch_count == 2) h.batch_stride = parts[k].rows / 2 * pitch;
+    }
+    for (int k = 0; k < count; k += 2) D8K_CUDA(launch_pad(ctx, dtype, jobs + k, count - k < 2 ? count - k : 2));
+    return 0;
+}
+
+int gated_grad_x(d8k_ctx* ctx, int dtype, void* dx, int rows, int xc, int yc, const GatedOperands& o, int accumulate) {
     GemmProblem g;  // the two products join one contraction: a batch of two that is summed
     g.dtype = dtype;
     g.M = rows; g.N = xc; g.K = yc;
-    g.a = matrix(dpre, false, yc, 2, 1LL * rows * yc);
-    g.b = matrix(w, false, yc, 2, 1LL * xc * yc);
+    g.a = o.dpre;
+    g.b = o.w;
     g.kbatch = 2;
     g.C = dx;
     g.ldc = xc;
     g.beta = accumulate ? 1 : 0;
+    g.ragged_k = true;
     return run_gemm(ctx, g);
 }
 
-int gated_grad_w(d8k_ctx* ctx, int dtype, const void* x, int xb, int xr, int xc, void* dw, int yc, const void* dpre, int accumulate) {
-    if (int rc = check_gated(0, xb, xr, xc, yc)) return rc;
-    const int rows = xb * xr;
-    const size_t es = esize(dtype), w_bytes = 2 * es * xc * yc;
-    if (!dw || (rows > 0 && (!x || !dpre))) return fail(D8K_ERR_ARGUMENT, "gated: null pointer");
-    if (rows == 0) {  // no row contributes
-        if (!accumulate) D8K_CUDA(cudaMemsetAsync(dw, 0, w_bytes, ctx->stream));
-        return 0;
-    }
-    if (overlap(dw, w_bytes, x, es * rows * xc) || overlap(dw, w_bytes, dpre, 2 * es * rows * yc)) return fail(D8K_ERR_ARGUMENT, "gated: dw overlaps an input");
+int gated_grad_w(d8k_ctx* ctx, int dtype, void* dw, int rows, int xc, int yc, const GatedOperands& o, int accumulate) {
     GemmProblem g;
     g.dtype = dtype;
     g.M = xc; g.N = yc; g.K = rows;
-    g.a = matrix(x, true, xc);
-    g.b = matrix(dpre, true, yc, 2, 1LL * rows * yc);
+    g.a = o.x;
+    g.b = o.dpre;
+    g.b.mn = true;
     g.batch = 2;
     g.C = dw;
     g.ldc = yc;
     g.c_batch_stride = 1LL * xc * yc;
     g.beta = accumulate ? 1 : 0;
+    g.ragged_k = true;
     return run_gemm(ctx, g);
 }
 
@@ -893,6 +960,44 @@ int rms_norm_backward(d8k_ctx* ctx, const T* x, const T* weight, const float* rs
 }
 
 }  // namespace
+
+bool rows_aligned(const void* ptr, long long ld, int dtype) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld * esize(dtype) % 16 == 0; }
+
+void* pad_memory(Ctx* ctx, size_t bytes) {
+    if (bytes <= ctx->pad_bytes) return ctx->pads.back();
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(ctx->stream, &capturing) != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    if (capturing != cudaStreamCaptureStatusNone) return nullptr;
+    size_t want = ctx->pad_bytes * 2 > bytes ? ctx->pad_bytes * 2 : bytes;  // the sum of all stays below twice the last
+    if (want < (static_cast<size_t>(16) << 20)) want = static_cast<size_t>(16) << 20;
+    ctx->pads.reserve(ctx->pads.size() + 1);
+    void* p = nullptr;
+    if (cudaMalloc(&p, want) != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    ctx->pads.push_back(p);
+    ctx->pad_bytes = want;
+    return p;
+}
+
+cudaError_t launch_pad(Ctx* ctx, int dtype, const PadJob* jobs, int count) {
+    PadJobs j;
+    size_t steps = 0;
+    for (int k = 0; k < count; ++k) {
+        j.job[k] = jobs[k];
+        steps += static_cast<size_t>(jobs[k].rows) * jobs[k].pitch * esize(dtype) / 16;
+    }
+    auto run = [&](auto kernel) { kernel<<<grid_for(static_cast<d8k_ctx*>(ctx), kernel, steps), 256, 0, ctx->stream>>>(j, count); };
+    if (dtype == D8K_F32) run(pad_kernel<float>);
+    else run(pad_kernel<__half>);
+    count_launch();
+    return cudaGetLastError();
+}
+
 }  // namespace d8k
 
 using namespace d8k;
@@ -931,35 +1036,71 @@ int d8k_gated_forward(d8k_ctx* ctx, int dtype, int activation, const void* x, in
 }
 
 int d8k_gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, const void* dz, void* dpre, size_t n, const d8k_dropout* drop) {
-    return entry(ctx, dtype, [&]() -> int { return gated_grad_pre(ctx, dtype, activation, pre, dz, dpre, n, drop); });
+    return entry(ctx, dtype, [&]() -> int { return gated_grad_pre(ctx, dtype, activation, pre, dz, dpre, n, 1, 1, drop); });
 }
 
 int d8k_gated_grad_x_into(d8k_ctx* ctx, int dtype, void* dx, int xb, int xr, int xc, const void* w, int yc, const void* dpre, int accumulate) {
-    return entry(ctx, dtype, [&]() -> int { return gated_grad_x(ctx, dtype, dx, xb, xr, xc, w, yc, dpre, accumulate); });
+    return entry(ctx, dtype, [&]() -> int {
+        if (int rc = check_gated(0, xb, xr, xc, yc)) return rc;
+        const int rows = xb * xr;
+        if (rows == 0) return 0;
+        if (!dx || !w || !dpre) return fail(D8K_ERR_ARGUMENT, "gated: null pointer");
+        const size_t es = esize(dtype), x_bytes = es * rows * xc;
+        if (overlap(dx, x_bytes, w, 2 * es * xc * yc) || overlap(dx, x_bytes, dpre, 2 * es * rows * yc))
+            return fail(D8K_ERR_ARGUMENT, "gated: dx overlaps an input");
+        GatedOperands o;
+        if (int rc = gated_operands(ctx, dtype, &o, nullptr, w, dpre, rows, xc, yc, false)) return rc;
+        return gated_grad_x(ctx, dtype, dx, rows, xc, yc, o, accumulate);
+    });
 }
 
 int d8k_gated_grad_w_into(d8k_ctx* ctx, int dtype, const void* x, int xb, int xr, int xc, void* dw, int yc, const void* dpre, int accumulate) {
-    return entry(ctx, dtype, [&]() -> int { return gated_grad_w(ctx, dtype, x, xb, xr, xc, dw, yc, dpre, accumulate); });
+    return entry(ctx, dtype, [&]() -> int {
+        if (int rc = check_gated(0, xb, xr, xc, yc)) return rc;
+        const int rows = xb * xr;
+        const size_t es = esize(dtype), w_bytes = 2 * es * xc * yc;
+        if (!dw || (rows > 0 && (!x || !dpre))) return fail(D8K_ERR_ARGUMENT, "gated: null pointer");
+        if (rows == 0) {  // no row contributes
+            if (!accumulate) D8K_CUDA(cudaMemsetAsync(dw, 0, w_bytes, ctx->stream));
+            return 0;
+        }
+        if (overlap(dw, w_bytes, x, es * rows * xc) || overlap(dw, w_bytes, dpre, 2 * es * rows * yc)) return fail(D8K_ERR_ARGUMENT, "gated: dw overlaps an input");
+        GatedOperands o;
+        if (int rc = gated_operands(ctx, dtype, &o, x, nullptr, dpre, rows, xc, yc, false)) return rc;
+        return gated_grad_w(ctx, dtype, dw, rows, xc, yc, o, accumulate);
+    });
 }
 
 int d8k_gated_backward(d8k_ctx* ctx, int dtype, int activation, const void* x, int xb, int xr, int xc, const void* w, int yc, const void* pre,
                        const void* dz, void* dpre, void* dx, void* dw, int accumulate, const d8k_dropout* drop) {
     return entry(ctx, dtype, [&]() -> int {
         if (int rc = check_gated(activation, xb, xr, xc, yc)) return rc;
-        const size_t es = esize(dtype), rows = static_cast<size_t>(xb) * xr;
-        if (rows > 0) {  // everything is checked before the first launch
-            if ((dx && !w) || (dw && !x)) return fail(D8K_ERR_ARGUMENT, "gated: null pointer");
-            const size_t xs = es * rows * xc, ws = 2 * es * xc * yc, hs = es * rows * yc;
-            if (overlap(dpre, 2 * hs, x, xs) || overlap(dpre, 2 * hs, w, ws) || overlap(dx, xs, x, xs) || overlap(dx, xs, w, ws) || overlap(dx, xs, pre, 2 * hs) ||
-                overlap(dx, xs, dz, hs) || overlap(dx, xs, dpre, 2 * hs) || overlap(dw, ws, x, xs) || overlap(dw, ws, w, ws) || overlap(dw, ws, pre, 2 * hs) ||
-                overlap(dw, ws, dz, hs) || overlap(dw, ws, dpre, 2 * hs) || overlap(dx, xs, dw, ws))
-                return fail(D8K_ERR_ARGUMENT, "gated: an output overlaps an input or another output");
+        const int rows = xb * xr;
+        const size_t es = esize(dtype), xs = es * rows * xc, ws = 2 * es * xc * yc, hs = es * rows * yc;
+        DropSpec spec;
+        int dropping = 0;
+        if (int rc = make_drop(drop, &spec, &dropping)) return rc;
+        if (rows == 0) {  // no row contributes
+            if (dw && !accumulate) D8K_CUDA(cudaMemsetAsync(dw, 0, ws, ctx->stream));
+            return 0;
         }
-        if (int rc = gated_grad_pre(ctx, dtype, activation, pre, dz, dpre, rows * yc, drop)) return rc;
+        // everything is checked before the first launch
+        if (!pre || !dz || !dpre || (dx && !w) || (dw && !x)) return fail(D8K_ERR_ARGUMENT, "gated: null pointer");
+        if ((dpre != pre && overlap(dpre, 2 * hs, pre, 2 * hs)) || overlap(dpre, 2 * hs, dz, hs) || overlap(dpre, 2 * hs, x, xs) || overlap(dpre, 2 * hs, w, ws) ||
+            overlap(dx, xs, x, xs) || overlap(dx, xs, w, ws) || overlap(dx, xs, pre, 2 * hs) || overlap(dx, xs, dz, hs) || overlap(dx, xs, dpre, 2 * hs) ||
+            overlap(dw, ws, x, xs) || overlap(dw, ws, w, ws) || overlap(dw, ws, pre, 2 * hs) || overlap(dw, ws, dz, hs) || overlap(dw, ws, dpre, 2 * hs) ||
+            overlap(dx, xs, dw, ws))
+            return fail(D8K_ERR_ARGUMENT, "gated: an output overlaps an input or another output");
+        GatedOperands o;
+        if (int rc = gated_operands(ctx, dtype, &o, dw ? x : nullptr, dx ? w : nullptr, dpre, rows, xc, yc, true)) return rc;
+        void* where = const_cast<void*>(o.dpre.ptr);
+        if (o.dpre.padded)  // the zeros behind each row
+            D8K_CUDA(cudaMemset2DAsync(static_cast<char*>(where) + es * yc, es * o.dpre.ld, 0, es * (o.dpre.ld - yc), 2 * static_cast<size_t>(rows), ctx->stream));
+        if (int rc = gated_grad_pre(ctx, dtype, activation, pre, dz, where, static_cast<size_t>(rows) * yc, yc, static_cast<size_t>(o.dpre.ld), drop)) return rc;
         if (dx)
-            if (int rc = gated_grad_x(ctx, dtype, dx, xb, xr, xc, w, yc, dpre, accumulate)) return rc;
+            if (int rc = gated_grad_x(ctx, dtype, dx, rows, xc, yc, o, accumulate)) return rc;
         if (dw)
-            if (int rc = gated_grad_w(ctx, dtype, x, xb, xr, xc, dw, yc, dpre, accumulate)) return rc;
+            if (int rc = gated_grad_w(ctx, dtype, dw, rows, xc, yc, o, accumulate)) return rc;
         return 0;
     });
 }

@@ -138,6 +138,12 @@ __device__ __forceinline__ void tc_commit_pair(uint32_t bar, uint16_t mask) {
 // touch every bank group once.
 __device__ __forceinline__ uint32_t slot_off(int r, int c16) { return static_cast<uint32_t>(r * 64 + ((c16 ^ ((r >> 1) & 3)) << 4)); }
 
+__device__ __forceinline__ __half ld_shared_half(uint32_t addr) {
+    unsigned short v;
+    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return __ushort_as_half(v);
+}
+
 struct PairWork {
     int batch, m0, n0;
 };
@@ -403,12 +409,33 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     }
                     const int col0 = it.n0 / 2 + c * 32;
                     if (col0 >= p.N) continue;
-                    if (!segments || col0 + 32 > p.N) {
-                        if (row < p.M) store_gated_chunk<OutT>(p, row, col0, gate, up);
-                        continue;
-                    }
                     const uint32_t s0 = staging, s1 = staging + Cfg::SLOT_BYTES;
                     using V = EpiVec<OutT>;
+                    if (!segments || col0 + 32 > p.N) {
+                        // rows that start anywhere, or end inside these columns: one row per store, a column per lane
+                        auto rows_out = [&](OutT* dst, uint32_t slot) {
+                            __syncwarp();
+#pragma unroll 4
+                            for (int rr = 0; rr < 32; ++rr)
+                                if (warp_row0 + rr < p.M && col0 + lane < p.N)
+                                    dst[static_cast<long long>(warp_row0 + rr) * p.ldc + col0 + lane] = ld_shared_half(s0 + slot + slot_off(rr, lane >> 3) + 2 * (lane & 7));
+                            __syncwarp();
+                        };
+                        if (t.pre) {
+#pragma unroll
+                            for (int v = 0; v < 4; ++v) {
+                                st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
+                                st_shared_v4(s1 + slot_off(lane, v), V::pack(up + 8 * v));
+                            }
+                            rows_out(reinterpret_cast<OutT*>(t.pre), 0);
+                            rows_out(reinterpret_cast<OutT*>(t.pre) + t.pre_stride, Cfg::SLOT_BYTES);
+                        }
+                        gated_values<OutT>(t, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0, gate, up);
+#pragma unroll
+                        for (int v = 0; v < 4; ++v) st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
+                        rows_out(reinterpret_cast<OutT*>(p.C), 0);
+                        continue;
+                    }
                     const long long first = static_cast<long long>(warp_row0) * p.ldc + col0 + lc * 8;  // this thread's piece of the segments
                     if (t.pre) {
 #pragma unroll

@@ -20,6 +20,10 @@ struct Ctx {
     unsigned epoch_counter = 0;  // this context's split launches so far, modulo 2^24 (GemmParams::epoch)
     unsigned* arrivals = nullptr;  // kMaxCounters words, zero between launches: kernels whose last CTA finishes the work count their CTAs here
     int* status = nullptr;     // device status word
+    // Memory for copies of operands with padded rows, grown as calls need it (pad_memory).  What a captured graph may point at is never freed
+    // before the context.
+    std::vector<void*> pads;
+    size_t pad_bytes = 0;  // of the last one
     GroupEntry* group_buf = nullptr;  // device memory for kMaxGroups entries of a grouped launch (null: launches are never grouped)
 };
 constexpr int kMaxCounters = 4096;
@@ -35,6 +39,7 @@ struct HostOperand {
     long long ld2 = 0;
     long long batch_stride = 0;
     int batch_count = 1;
+    bool padded = false;       // a stored matrix whose rows go on as zeros to the next multiple of 128 bytes (pad_operands)
     ConvRule cr = {};
     // halo != 0 (set by run_gemm, fp32 only): the virtual matrix is fetched as per-tile patches of halo_rows x halo_wp pixels
     int halo = 0, halo_wp = 0, halo_rows = 0;
@@ -59,6 +64,7 @@ struct GemmProblem {
     float epi_a = 0.f, epi_b = 0.f;
     void* E1 = nullptr;
     void* E2 = nullptr;
+    bool ragged_k = false;   // the paired kernel may also take a contraction that ends inside a k-block (see make_plan)
     int force_splits = 0;    // > 0: this many splits (bounded by the k-block count and the scratch) instead of the plan's own choice
     int ticket_base = 0;     // first of the context's tickets this launch uses (grouped launches give every contraction its own range)
     bool ws_strict = false;  // split within ws / ws_bytes, never in the context's own scratch (run_gemm_group carves that up itself)
@@ -70,6 +76,20 @@ struct GemmProblem {
     void* scatter_base[kMaxScatter] = {};
     OutMap out = {};  // strided placement of rows / columns in the output tensor (GemmParams::out); FastDivs filled by run_gemm
 };
+
+// A row-major matrix stack to copy with its rows padded by zeros to whole 128-byte pieces
+struct PadJob {
+    const void* src = nullptr;
+    void* dst = nullptr;
+    long long rows = 0;  // of all matrices of the stack
+    int cols = 0, pitch = 0;
+};
+// `bytes` of the context's padding memory, 256-byte aligned; null when it is smaller and the stream is being captured, or no more is to be had
+void* pad_memory(Ctx* ctx, size_t bytes);
+// up to two copies in one launch (feedforward.cu)
+cudaError_t launch_pad(Ctx* ctx, int dtype, const PadJob* jobs, int count);
+// whether TMA can describe a stored matrix stack of rows of `ld` elements at ptr
+bool rows_aligned(const void* ptr, long long ld, int dtype);
 
 // act(A B[0]) * (A B[1]) for row-major A [M, K] and B [2, K, N] (GemmCfg::GATED); C [M, N]
 struct GatedProblem {

@@ -85,7 +85,7 @@ bool make_pair_map(CUtensorMap* map, const HostOperand& o, long long extent, lon
     if (!enc) return false;
     const long long ce = 128 / esize;
     long long rows = o.mn ? K : extent;           // stored rows
-    long long groups = (o.mn ? extent : K) / ce;  // 128-byte groups along the stored row
+    long long groups = ((o.mn ? extent : K) + (o.padded ? ce - 1 : 0)) / ce;  // 128-byte groups along the stored row
     cuuint64_t dims[4] = {static_cast<cuuint64_t>(ce), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(groups),
                           static_cast<cuuint64_t>(o.batch_count)};
     long long bstride = o.batch_count > 1 ? o.batch_stride : rows * o.ld;
@@ -308,7 +308,7 @@ Plan make_plan(const Ctx* ctx, const GemmProblem& g, size_t scratch_limit) {
     pl.tma = pl.a_tma >= 0 && pl.b_tma >= 0 && encode_tiled() != nullptr && !env_int("D8K_FORCE_GATHER", 0);
     if ((pl.a_tma > kTmaTiled || pl.b_tma > kTmaTiled) && !env_int("D8K_IM2COL", 1)) pl.tma = false;
     // fp32 behind TMA: an MN-major stored matrix arrives as one box of whole 32-element chunks
-    if (pl.f32 && ((pl.a_tma == kTmaTiled && g.a.mn && g.M % 32 != 0) || (pl.b_tma == kTmaTiled && g.b.mn && g.N % 32 != 0) ||
+    if (pl.f32 && ((pl.a_tma == kTmaTiled && g.a.mn && g.M % 32 != 0 && !g.a.padded) || (pl.b_tma == kTmaTiled && g.b.mn && g.N % 32 != 0 && !g.b.padded) ||
                    !env_int("D8K_F32_TMA", 1)))
         pl.tma = false;
     if (pl.f32) pl.bn = 64;  // the 64-column fp32 kernels run two groups of helper warps (see GemmCfg::LOADER_GROUPS)
@@ -353,7 +353,10 @@ Plan make_plan(const Ctx* ctx, const GemmProblem& g, size_t scratch_limit) {
     // CTA pairs on 256 x 256 tiles once the output alone fills the machine (74 pairs) and nothing is split
     int tiles256 = g.batch * ((g.M + 255) / 256) * ((g.N + 255) / 256);
     pl.pair = pl.tma && pl.a_tma == kTmaTiled && pl.b_tma == kTmaTiled && !g.out.rows_on && !g.out.cols_on && pl.bn == 256 && pl.splits == 1 && (tiles256 * 2 >= ctx->num_sms || pair_early(ctx, g) || env_int("D8K_PAIR", 1) == 2) && env_int("D8K_PAIR", 1) != 0 &&
-              g.K % 64 == 0 && (!g.a.mn || g.M % 64 == 0) && (!g.b.mn || g.N % 64 == 0);
+              // whole 64-element groups of each stored row, or rows padded to them.  An MN-major operand's k are rows, which end
+              // anywhere (what a box holds beyond is zeros); only ragged_k problems use that, the others keep the kernel they had
+              (g.K % 64 == 0 || (g.ragged_k && (g.a.mn || g.a.padded) && (g.b.mn || g.b.padded))) &&
+              (!g.a.mn || g.M % 64 == 0 || g.a.padded) && (!g.b.mn || g.N % 64 == 0 || g.b.padded);
     if (pl.pair) {
         pl.tiles_m = (g.M + 255) / 256;
         pl.tiles_n = (g.N + 255) / 256;
@@ -566,7 +569,7 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
             if (mode == kTmaFilterSub) return make_filter_sub_map(map, o, rows_tile, esize, false, atom32);
             if (mode == kTmaFilterTapSub) return make_filter_sub_map(map, o, rows_tile, esize, true, atom32);
             if (!o.mn) return make_map(map, o, g.K, extent, rows_tile, esize);
-            *chunked = (pl.f32 || extent % ce == 0) && env_int("D8K_CHUNKED", 1);
+            *chunked = (pl.f32 || extent % ce == 0 || o.padded) && env_int("D8K_CHUNKED", 1);
             if (pl.f32 && !*chunked) return false;
             return *chunked ? make_pair_map(map, o, extent, g.K, ce, rows_tile / ce, esize, atom32) : make_map(map, o, extent, g.K, ce, esize);
         };
@@ -674,8 +677,8 @@ static int run_gated_few(Ctx* ctx, const GatedProblem& g, const HostOperand& x, 
     p.kb_per_split = (p.num_kb + splits - 1) / splits;
     p.splits = (p.num_kb + p.kb_per_split - 1) / p.kb_per_split;
     p.total_work = strips * p.splits;
-    p.x_chunked = g.K % 64 == 0;
-    p.w_chunked = g.N % 64 == 0;
+    p.x_chunked = g.K % 64 == 0 || x.padded;
+    p.w_chunked = g.N % 64 == 0 || w.padded;
     p.status = ctx->status;
     p.h = g.C;
     p.gated = g.tail;
@@ -706,11 +709,48 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     b.ld = g.N;
     b.batch_count = 2;
     b.batch_stride = static_cast<long long>(g.K) * g.N;
-    const bool tma = tma_ok(a, esize) && tma_ok(b, esize) && encode_tiled() != nullptr && !env_int("D8K_FORCE_GATHER", 0);
+    const bool can_tma = encode_tiled() != nullptr && !env_int("D8K_FORCE_GATHER", 0);
+    if (can_tma && !(tma_ok(a, esize) && tma_ok(b, esize))) {
+        // Rows that do not start on 16-byte boundaries: copies with padded rows, read by TMA.  The loader warps fetch such rows element by
+        // element (333 x 250 x 1001 fp32: 40 us).
+        PadJob jobs[2];
+        int count = 0;
+        size_t bytes = 0;
+        auto plan = [&](HostOperand& o, long long rows, int cols) {
+            if (tma_ok(o, esize)) return;
+            PadJob& j = jobs[count++];
+            j.src = o.ptr;
+            j.rows = rows;
+            j.cols = cols;
+            j.pitch = (cols + bk - 1) / bk * bk;
+            j.dst = reinterpret_cast<void*>(bytes);
+            bytes += (static_cast<size_t>(rows) * j.pitch * esize + 255) & ~static_cast<size_t>(255);
+        };
+        plan(a, g.M, g.K);
+        const bool a_copied = count == 1;
+        plan(b, 2LL * g.K, g.N);
+        if (char* base = static_cast<char*>(pad_memory(ctx, bytes))) {
+            for (int k = 0; k < count; ++k) jobs[k].dst = base + reinterpret_cast<size_t>(jobs[k].dst);
+            if (cudaError_t e = launch_pad(ctx, g.dtype, jobs, count)) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
+            if (a_copied) {
+                a.ptr = jobs[0].dst;
+                a.ld = jobs[0].pitch;
+                a.padded = true;
+            }
+            if (count == (a_copied ? 2 : 1)) {
+                const PadJob& j = jobs[count - 1];
+                b.ptr = j.dst;
+                b.ld = j.pitch;
+                b.batch_stride = static_cast<long long>(g.K) * j.pitch;
+                b.padded = true;
+            }
+        }
+    }
+    const bool tma = can_tma && tma_ok(a, esize) && tma_ok(b, esize);
     if (tma && !f32 && g.M <= 128) return run_gated_few(ctx, g, a, b);
     const long long mtiles = (g.M + kBM - 1) / kBM, ptiles = (g.M + 255LL) / 256 * ((g.N + 127) / 128);
     // The paired kernel from half a wave of its tiles on, with a long contraction from a third of one, as in make_plan.
-    const bool pair = tma && !f32 && g.K % 64 == 0 && g.N % 64 == 0 && env_int("D8K_PAIR", 1) != 0 &&
+    const bool pair = tma && !f32 && (g.K % 64 == 0 || a.padded) && (g.N % 64 == 0 || b.padded) && env_int("D8K_PAIR", 1) != 0 &&
                       (ptiles * 2 >= ctx->num_sms || (g.K >= 2048 && ptiles * 3 >= ctx->num_sms));
     int bn = f32 ? 64 : 128;
     if (!f32 && tma && mtiles * ((g.N + 127) / 128) >= ctx->num_sms) bn = 256;  // wide tiles when they alone give every SM one
@@ -762,7 +802,7 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
         form = "pair";
     } else if (tma) {
         p.a_tma = p.b_tma = kTmaTiled;
-        p.b_chunked = !f32 && g.N % bk == 0;  // each projection's columns of a tile as one box
+        p.b_chunked = !f32 && (g.N % bk == 0 || b.padded);  // each projection's columns of a tile as one box
         if (!make_map(&ta, a, g.K, g.M, kBM, esize) ||
             !(p.b_chunked ? make_pair_map(&tb, b, g.N, g.K, bk, bn / 2 / bk, esize) : make_map(&tb, b, g.N, g.K, bk, esize, f32)))
             return fail(2, "gated: cuTensorMapEncodeTiled failed");

@@ -303,7 +303,11 @@ D8K_API int d8k_gated_grad_x_into(d8k_ctx* ctx, int dtype, void* dx, int xb, int
 /* dw[b] (+)= x^T * dpre[b], one launch for both. */
 D8K_API int d8k_gated_grad_w_into(d8k_ctx* ctx, int dtype, const void* x, int xb, int xr, int xc, void* dw, int yc, const void* dpre,
                                   int accumulate);
-/* The three above: dpre (2 x rows x yc, workspace; may be pre) from pre and dz, then dx and dw; dx or dw may be NULL. */
+/* The three above: dpre from pre and dz, then dx and dw; dx or dw may be NULL.  dpre (2 x rows x yc) is workspace, its contents afterwards
+ * unspecified; it may be pre, which is then overwritten.
+ * Rows that do not start on 16-byte boundaries (an odd xc or yc) are copied with padding before these products and d8k_gated_forward read
+ * them: the first call of a size may allocate the copies' memory, which the context keeps; make it before any stream capture (inside
+ * one, slower kernels that need no copies run instead when the memory is not there). */
 D8K_API int d8k_gated_backward(d8k_ctx* ctx, int dtype, int activation, const void* x, int xb, int xr, int xc, const void* w, int yc,
                                const void* pre, const void* dz, void* dpre, void* dx, void* dw, int accumulate, const d8k_dropout* drop);
 

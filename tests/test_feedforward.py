@@ -139,7 +139,7 @@ def check_gated(x, w, name, h, pre, drop=None):
 # boundaries, enough tiles for every tile shape of the fp16 kernels, contractions that are split
 GATED = [((1, 1, 1), 1), ((1, 1, 64), 64), ((1, 3, 17), 9), ((2, 65, 40), 72), ((1, 129, 128), 192), ((1, 257, 130), 250), ((3, 100, 64), 1000),
          ((1, 1, 4096), 512), ((1, 7, 2048), 1032), ((1, 48, 1600), 264), ((1, 127, 1000), 504), ((1, 300, 512), 520)]
-GATED_LARGE = [((1, 1500, 512), 2496), ((2, 1024, 320), 4992), ((1, 2047, 128), 2504), ((1, 1300, 72), 2002)]
+GATED_LARGE = [((1, 1500, 512), 2496), ((2, 1024, 320), 4992), ((1, 2047, 128), 2504), ((1, 1300, 72), 2002), ((1, 1999, 333), 2503)]
 
 
 # ------------------------------------------------------------------------------------------------ on the CPU
@@ -412,7 +412,7 @@ def check_backward(x, w, pre, dz, dx, dw, name, drop, dx0=None, dw0=None):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", GATED + GATED_LARGE[:1], ids=str)
+@pytest.mark.parametrize("shape", GATED + GATED_LARGE, ids=str)
 def test_gated_backward(ctx, shape, dtype):
     (xb, xr, xc), yc = shape
     x, w = tensor(13, (xb, xr, xc), dtype), tensor(14, (2, xc, yc), dtype, 1.0 / math.sqrt(xc))
@@ -736,6 +736,48 @@ def test_block_captured_and_replayed(dtype):
         assert int(counter) == 3
     assert c.status() == 0
     del graphs
+    c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_odd_rows_captured(dtype):
+    """Sizes whose rows are copied with padding: captured in a context that has no memory for the copies yet (kernels without copies run),
+    then eagerly (the memory comes), then captured again, then a larger size while the older graph, which reads the older memory,
+    is still replayed."""
+    import deep8_b200
+    c = deep8_b200.Context(0)
+    side = torch.cuda.Stream()
+    c.use_stream(side)
+    sizes = [(70, 51, 133), (300, 1001, 2003)]
+    with torch.cuda.stream(side):
+        held = []
+        for rows, cols, width in sizes:
+            x, w = tensor(1, (1, rows, cols), dtype), tensor(2, (2, cols, width), dtype, cols ** -0.5)
+            pre, dz = tensor(3, (2, rows, width), dtype), tensor(4, (1, rows, width), dtype, 0.1)
+            for eager_first in (False, True):
+                h, kept, dx, dw, dpre = (torch.empty_like(t) for t in (dz, pre, x, w, pre))
+
+                def step():
+                    c.gated_forward(x, w, "silu", out=h, pre=kept)
+                    c.gated_backward(x, w, pre, dz, dx, dw, "silu", dpre=dpre, accumulate=False)
+
+                if eager_first:
+                    step()
+                side.synchronize()
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=side):
+                    step()
+                held.append((g, x, w, pre, dz, h, kept, dx, dw))
+            for g, x, w, pre, dz, h, kept, dx, dw in held:
+                for t in (h, kept, dx, dw):
+                    t.fill_(float("nan"))
+                g.replay()
+                side.synchronize()
+                check_gated(x, w, "silu", h, kept)
+                check_backward(x, w, pre, dz, dx, dw, "silu", None)
+    assert c.status() == 0
+    del held, g
     c.close()
 
 
