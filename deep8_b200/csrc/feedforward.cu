@@ -820,7 +820,7 @@ int gated_grad_x(d8k_ctx* ctx, int dtype, void* dx, int rows, int xc, int yc, co
     g.ldc = xc;
     g.beta = accumulate ? 1 : 0;
     g.ragged_k = true;
-    return run_gemm(ctx, g);
+    return run_gemm_long(ctx, g);
 }
 
 int gated_grad_w(d8k_ctx* ctx, int dtype, void* dw, int rows, int xc, int yc, const GatedOperands& o, int accumulate) {
@@ -836,7 +836,7 @@ int gated_grad_w(d8k_ctx* ctx, int dtype, void* dw, int rows, int xc, int yc, co
     g.c_batch_stride = 1LL * xc * yc;
     g.beta = accumulate ? 1 : 0;
     g.ragged_k = true;
-    return run_gemm(ctx, g);
+    return run_gemm_long(ctx, g);
 }
 
 int dropout(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* y, size_t n, const d8k_dropout* drop) {

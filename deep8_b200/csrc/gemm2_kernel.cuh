@@ -28,8 +28,11 @@
 
 namespace d8k {
 
-template <bool A_MN_, bool B_MN_, int STAGES_, int SUB_ = 2, bool GATED_ = false>
+template <bool A_MN_, bool B_MN_, int STAGES_, int SUB_ = 2, bool GATED_ = false, bool SPLIT_ = false>
 struct Gemm2Cfg {
+    // SPLIT: a work item is a tile and one of p.splits slices of the contraction (p.kb_per_split stages each); the epilogue stores the fp32
+    // accumulator as it is, and split_sum_kernel adds the slices.
+    static constexpr bool SPLIT = SPLIT_;
     // GATED (see GemmCfg): CTA 0 of the pair stages 128 columns of the gate projection, CTA 1 the same columns of the up projection; the
     // accumulator's columns [0, 128) are the gate's, [128, 256) the up projection's, for a tile of 256 x 128 outputs.
     static constexpr bool GATED = GATED_;
@@ -46,7 +49,7 @@ struct Gemm2Cfg {
     static constexpr int TMEM_COLS = 512;        // two accumulator buffers of 256 columns
     // GATED: eight epilogue warps (0-3 and 6-9), two for each quarter of the accumulator's rows, each half of the columns: the activation
     // makes the epilogue several times longer than a plain store, and with four warps it outlasted a K = 4096 tile's main loop
-    static constexpr int EPI_WARPS = GATED ? 8 : 4, PRODUCER_WARP = 4, MMA_WARP = 5;
+    static constexpr int EPI_WARPS = GATED && !SPLIT ? 8 : 4, PRODUCER_WARP = 4, MMA_WARP = 5;
     static constexpr int THREADS = 32 * (EPI_WARPS + 2);
     static constexpr int BAR_BYTES = 256;
     // epilogue staging: per epilogue warp three slots (C, E1, E2) of 32 rows x 64 bytes (32 fp16 columns)
@@ -235,10 +238,11 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const bool hinted = (p.l2_a | p.l2_b) != 0;
         const uint64_t pol_a = ptx::l2_policy(p.l2_a), pol_b = ptx::l2_policy(p.l2_b);
         for (int w = pair; ok && w < p.total_work; w += num_pairs) {
-            PairWork it = decode_pair_work(p, w);
+            PairWork it = decode_pair_work(p, Cfg::SPLIT ? w / p.splits : w);
+            const int kk_begin = Cfg::SPLIT ? w % p.splits * p.kb_per_split : 0, kk_end = Cfg::SPLIT ? min(total_it, kk_begin + p.kb_per_split) : total_it;
             const int my_m0 = it.m0 + 128 * static_cast<int>(rank);
             const int my_n0 = Cfg::GATED ? it.n0 / 2 : it.n0 + Cfg::HALF_N * static_cast<int>(rank);
-            for (int kk = 0; kk < total_it; ++kk) {
+            for (int kk = kk_begin; kk < kk_end; ++kk) {
                 const long long tw = p.prof ? clock64() : 0;
                 ok = wait_bar(empty_bar(stage), phase ^ 1, &s_abort, p.status, (kRoleProducer << 8) | 1);
                 if (!ok) break;
@@ -296,7 +300,8 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 if (p.prof) waited_tmem += clock64() - tt;
                 ptx::tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + acc * 256;
-                for (int kk = 0; kk < total_it; ++kk) {
+                const int kk_begin = Cfg::SPLIT ? w % p.splits * p.kb_per_split : 0, kk_end = Cfg::SPLIT ? min(total_it, kk_begin + p.kb_per_split) : total_it;
+                for (int kk = kk_begin; kk < kk_end; ++kk) {
                     const long long tw = p.prof ? clock64() : 0;
                     ok = wait_bar(full_bar(stage), phase, &s_abort, p.status, (kRoleMma << 8) | 1);
                     if (!ok) break;
@@ -307,10 +312,10 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         for (int s = 0; s < Cfg::KSTEPS; ++s) {
                             uint64_t da = ptx::smem_desc(stage_a(stage) + a_off(s), a_lbo, 1024, ptx::kLayoutSw128);
                             uint64_t db = ptx::smem_desc(stage_b(stage) + b_off(s), b_lbo, 1024, ptx::kLayoutSw128);
-                            ptx::mma_f16_pair(d_tmem, da, db, idesc, (kk > 0 || s > 0) ? 1u : 0u);
+                            ptx::mma_f16_pair(d_tmem, da, db, idesc, (kk > kk_begin || s > 0) ? 1u : 0u);
                         }
                         ptx::tc_commit_pair(empty_bar(stage), 3);
-                        if (kk + 1 == total_it) ptx::tc_commit_pair(tfull_bar(acc), 3);
+                        if (kk + 1 == kk_end) ptx::tc_commit_pair(tfull_bar(acc), 3);
                     }
                     __syncwarp();
                     if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -323,7 +328,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 p.prof[blockIdx.x * 8 + 4] = waited_tmem;
             }
         }
-    } else if (warp < 4 || Cfg::GATED) {
+    } else if (warp < 4 || Cfg::EPI_WARPS == 8) {
         // ============================================================================ epilogue (both CTAs, own rows)
         using OutT = __half;
         const int quarter = warp & 3;  // the accumulator lanes this warp may read
@@ -341,7 +346,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         long long waited = 0;
         const long long t_begin = p.prof ? clock64() : 0;
         for (int w = pair; ok && w < p.total_work; w += num_pairs) {
-            PairWork it = decode_pair_work(p, w);
+            PairWork it = decode_pair_work(p, Cfg::SPLIT ? w / p.splits : w);
             const int row = it.m0 + 128 * static_cast<int>(rank) + row_in_tile;
             const long long crow = static_cast<long long>(it.batch) * p.c_batch_stride + static_cast<long long>(row) * p.ldc + scatter_offset(p, row);
             const int warp_row0 = it.m0 + 128 * static_cast<int>(rank) + quarter * 32;  // first row of this warp
@@ -386,7 +391,21 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             if (p.prof) waited += clock64() - tw;
             ptx::tc_fence_after_sync();
             const uint32_t taddr = tmem_base + acc * 256 + (static_cast<uint32_t>(quarter * 32) << 16);
-            if constexpr (Cfg::GATED) {
+            if constexpr (Cfg::SPLIT) {
+                const int tile = (it.batch * p.tiles_m + it.m0 / 256) * p.tiles_n + it.n0 / 256, tiles = p.batch * p.tiles_m * p.tiles_n;
+                float* part = p.ws + ((static_cast<size_t>(w % p.splits) * tiles + tile) * 256 + 128 * rank + row_in_tile) * 256;
+#pragma unroll 1
+                for (int c = 0; c < 256 / 32; ++c) {
+                    uint32_t r[32];
+                    __syncwarp();
+                    ptx::tmem_ld_32x32(taddr + c * 32, r);
+                    ptx::tmem_ld_wait();
+                    if (row < p.M) {
+#pragma unroll
+                        for (int v = 0; v < 8; ++v) __stcg(reinterpret_cast<uint4*>(part + c * 32) + v, make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]));
+                    }
+                }
+            } else if constexpr (Cfg::GATED) {
                 // 32 columns of both projections at a time; the projections (when kept) and then h cross to whole row segments through
                 // the warp's two staging slots
                 const GatedTail& t = p.gated;
@@ -468,7 +487,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 }
             }
 #pragma unroll 1
-            for (int c = 0; c < (Cfg::GATED ? 0 : 256 / 32); ++c) {
+            for (int c = 0; c < (Cfg::GATED || Cfg::SPLIT ? 0 : 256 / 32); ++c) {
                 uint32_t r[32];
                 __syncwarp();
                 ptx::tmem_ld_32x32(taddr + c * 32, r);

@@ -101,6 +101,17 @@ struct GatedProblem {
     GatedTail tail = {};
 };
 
+// Sum of a split paired product's slices, with the gated tail or an (accumulating) store (gemm_inst_gated_pair.cu)
+struct SplitSum {
+    const float* ws;
+    int splits, batch, tiles_m, tiles_n, M, N;
+    void* C;
+    long long ldc, c_batch_stride;
+    int beta;
+    GatedTail gated;
+};
+cudaError_t launch_split_sum(const Ctx* ctx, const SplitSum& q, bool gated);
+
 // the kernel for a few rows (gemm_gated_few.cu)
 struct GatedFewParams {
     int rows, width;
@@ -137,6 +148,8 @@ struct PreparedGemm {
 int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture = nullptr);
 // The gated pair of products as one launch; every extent at least 1, every pointer checked by the caller
 int run_gated(Ctx* ctx, const GatedProblem& g);
+// run_gemm, or the split paired kernel where that is the faster one: fp16 products with a long contraction and few output tiles
+int run_gemm_long(Ctx* ctx, const GemmProblem& g);
 // The contractions of one operator (the residue classes of a strided convolution): ONE launch whose work items are all of
 // theirs when the context has a group buffer and every part runs the same one-CTA-per-SM kernel, otherwise one launch each.
 int run_gemm_group(Ctx* ctx, std::vector<GemmProblem>& parts);
@@ -159,6 +172,9 @@ GemmLaunchFn lookup_f16_gated(int bn);
 GemmLaunchFn lookup_f32_gated(int mode);
 GemmLaunchFn lookup_gated_gather(bool f32);  // loader warps: 128 columns fp16, 64 fp32
 GemmLaunchFn lookup_f16_gated_pair();
+// the same and the plain paired kernel on slices of the contraction (Gemm2Cfg::SPLIT)
+GemmLaunchFn lookup_f16_gated_pair_split();
+GemmLaunchFn lookup_f16_pair_split(bool a_mn, bool b_mn);
 // paired-CTA kernel: the first argument of the launch function is the number of CTA pairs
 GemmLaunchFn lookup_f16_pair(bool a_mn, bool b_mn);
 

@@ -655,6 +655,96 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
     return 0;
 }
 
+// How many slices the paired kernel should cut a contraction of `its` stages (of 128 k) into, 0 when the ordinary kernels are faster.  The model,
+// in us, from measured times: a stage of a 256 x 256 tile 0.76, a launch with its fill and drain 6; the sum's launch 3 and its reads at 3 TB/s; a
+// k-block of 64 on the one-CTA kernel's 128 x 128 tile 0.5, whatever it multiplies.  `tiles` counts 256 x 256 tiles, `singles` the
+// one-CTA kernel's.
+static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int its, bool pair_fits_unsplit) {
+    const int pairs = ctx->num_sms / 2;
+    const double unsplit = (tiles + pairs - 1) / pairs * its * 0.76 + 6;
+    // the one-CTA kernel splits, too, when its tiles leave half of the SMs idle: at least 24 k-blocks each
+    double single_kb = 2.0 * its, extra = 0;
+    if (singles * 2 <= ctx->num_sms) {
+        long long s = ctx->num_sms / singles;
+        if (s > its / 12) s = its / 12;
+        if (s > 1) {
+            single_kb /= s;
+            extra = 4;
+        }
+    }
+    double best = (singles + ctx->num_sms - 1) / ctx->num_sms * single_kb * 0.5 + 6 + extra;
+    if (pair_fits_unsplit && unsplit < best) best = unsplit;
+    int slices = 0;
+    for (int s = 1; s <= its && s <= 32; ++s) {
+        const int per = (its + s - 1) / s;
+        if ((its + per - 1) / per != s) continue;
+        const double bytes = static_cast<double>(tiles) * s * 65536 * 4;
+        if (bytes > static_cast<double>(ctx->scratch_bytes)) break;
+        const double t = (tiles * s + pairs - 1) / pairs * per * 0.76 + 6 + 3 + bytes / 3e6;
+        if (t < best) {
+            best = t;
+            slices = s;
+        }
+    }
+    return slices;
+}
+
+int run_gemm_long(Ctx* ctx, const GemmProblem& g) {
+    const bool whole = (g.K % 64 == 0 || ((g.a.mn || g.a.padded) && (g.b.mn || g.b.padded))) && (!g.a.mn || g.M % 64 == 0 || g.a.padded) &&
+                       (!g.b.mn || g.N % 64 == 0 || g.b.padded);
+    if (g.dtype != 0 || !whole || !tma_ok(g.a, 2) || !tma_ok(g.b, 2) || encode_tiled() == nullptr || !env_int("D8K_PAIR", 1) || env_int("D8K_FORCE_GATHER", 0))
+        return run_gemm(ctx, g);
+    const long long tiles_m = (g.M + 255LL) / 256, tiles_n = (g.N + 255LL) / 256, tiles = g.batch * tiles_m * tiles_n;
+    const long long singles = static_cast<long long>(g.batch) * ((g.M + 127LL) / 128) * ((g.N + 127LL) / 128);
+    const int num_kb = (g.K + 63) / 64, its = g.kbatch * ((num_kb + 1) / 2);
+    const int slices = tiles > 4 * ctx->num_sms ? 0 : pair_slices(ctx, tiles, singles, its, tiles * 2 >= ctx->num_sms);
+    if (slices == 0) return run_gemm(ctx, g);
+    GemmParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.M = g.M; p.N = g.N; p.K = g.K;
+    p.batch = g.batch;
+    p.kbatch = g.kbatch;
+    p.num_kb = num_kb;
+    p.splits = slices;
+    p.kb_per_split = (its + slices - 1) / slices;
+    p.tiles_m = static_cast<int>(tiles_m);
+    p.tiles_n = static_cast<int>(tiles_n);
+    p.raster_group = 16;
+    p.total_work = static_cast<int>(tiles) * slices;
+    p.ws = ctx->scratch;
+    p.status = ctx->status;
+    p.a_batch_mod = g.a.batch_count;
+    p.b_batch_mod = g.b.batch_count;
+    CUtensorMap ta, tb;
+    std::memset(&ta, 0, sizeof(ta));
+    std::memset(&tb, 0, sizeof(tb));
+    if (!make_pair_map(&ta, g.a, g.M, g.K) || !make_pair_map(&tb, g.b, g.N, g.K)) return fail(2, "gemm: cuTensorMapEncodeTiled (4-D) failed");
+    const int pairs = p.total_work < ctx->num_sms / 2 ? p.total_work : ctx->num_sms / 2;
+    cudaError_t e = lookup_f16_pair_split(g.a.mn, g.b.mn)(pairs, ctx->stream, ta, tb, p);
+    if (e != cudaSuccess) return fail(2, std::string("gemm: launch failed: ") + cudaGetErrorString(e));
+    count_launch();
+    SplitSum q;
+    std::memset(&q, 0, sizeof(q));
+    q.ws = ctx->scratch;
+    q.splits = slices;
+    q.batch = g.batch;
+    q.tiles_m = p.tiles_m;
+    q.tiles_n = p.tiles_n;
+    q.M = g.M;
+    q.N = g.N;
+    q.C = g.C;
+    q.ldc = g.ldc;
+    q.c_batch_stride = g.c_batch_stride;
+    q.beta = g.beta;
+    e = launch_split_sum(ctx, q, false);
+    if (e != cudaSuccess) return fail(2, std::string("gemm: launch failed: ") + cudaGetErrorString(e));
+    count_launch();
+    std::ostringstream os;
+    os << "f16 pair slices=" << slices << " grid=" << pairs;
+    set_last_kernel(os.str());
+    return 0;
+}
+
 // The kernel for up to 128 rows of fp16 (gemm_gated_few.cu).
 static int run_gated_few(Ctx* ctx, const GatedProblem& g, const HostOperand& x, const HostOperand& w) {
     GatedFewParams p;
@@ -752,9 +842,14 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     // The paired kernel from half a wave of its tiles on, with a long contraction from a third of one, as in make_plan.
     const bool pair = tma && !f32 && (g.K % 64 == 0 || a.padded) && (g.N % 64 == 0 || b.padded) && env_int("D8K_PAIR", 1) != 0 &&
                       (ptiles * 2 >= ctx->num_sms || (g.K >= 2048 && ptiles * 3 >= ctx->num_sms));
+    // a long contraction with few tiles: slices on the paired kernel
+    const int its = (g.K + 127) / 128;
+    int slices = 0;
+    if (tma && !f32 && (g.K % 64 == 0 || a.padded) && (g.N % 64 == 0 || b.padded) && env_int("D8K_PAIR", 1) != 0 && ptiles <= 4 * ctx->num_sms)
+        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, pair);
     int bn = f32 ? 64 : 128;
     if (!f32 && tma && mtiles * ((g.N + 127) / 128) >= ctx->num_sms) bn = 256;  // wide tiles when they alone give every SM one
-    const long long tiles = pair ? ptiles : mtiles * ((g.N + bn / 2 - 1) / (bn / 2));
+    const long long tiles = pair || slices ? ptiles : mtiles * ((g.N + bn / 2 - 1) / (bn / 2));
     if (tiles >= (1LL << 30)) return fail(1, "the shape is too large");
 
     GemmParams p;
@@ -762,11 +857,11 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     p.M = g.M; p.N = g.N; p.K = g.K;
     p.batch = p.kbatch = 1;
     p.num_kb = (g.K + bk - 1) / bk;
-    p.tiles_m = static_cast<int>(pair ? (g.M + 255LL) / 256 : mtiles);
+    p.tiles_m = static_cast<int>(pair || slices ? (g.M + 255LL) / 256 : mtiles);
     p.tiles_n = static_cast<int>(tiles / p.tiles_m);
     p.raster_group = 16;
     int splits = 1;  // as in make_plan: at least 24 k-blocks per split
-    if (!pair && tiles * 2 <= ctx->num_sms && tiles <= kMaxCounters) {
+    if (!pair && !slices && tiles * 2 <= ctx->num_sms && tiles <= kMaxCounters) {
         splits = ctx->num_sms / static_cast<int>(tiles);
         if (splits > p.num_kb / 24) splits = p.num_kb / 24;
         const size_t per_split = static_cast<size_t>(tiles) * kBM * bn * sizeof(float);
@@ -792,7 +887,15 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     GemmLaunchFn fn = nullptr;
     int resident = ctx->num_sms;  // work items in flight together
     const char* form = "gather";
-    if (pair) {
+    if (slices) {
+        if (!make_pair_map(&ta, a, g.M, g.K) || !make_pair_map(&tb, b, g.N, g.K)) return fail(2, "gated: cuTensorMapEncodeTiled (4-D) failed");
+        p.splits = slices;
+        p.kb_per_split = (its + slices - 1) / slices;
+        p.total_work = static_cast<int>(tiles) * slices;
+        fn = lookup_f16_gated_pair_split();
+        resident = ctx->num_sms / 2;
+        form = "pair slices";
+    } else if (pair) {
         if (!make_pair_map(&ta, a, g.M, g.K) || !make_pair_map(&tb, b, g.N, g.K)) return fail(2, "gated: cuTensorMapEncodeTiled (4-D) failed");
         const Raster r = pick_raster(g.M, 2LL * g.N, g.K, p.tiles_m, p.tiles_n, ctx->num_sms / 2);
         p.raster_group = r.group;
@@ -824,12 +927,29 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     }
     if (!fn) return fail(2, "gated: no kernel for this configuration");
     const int grid = p.total_work < resident ? p.total_work : resident;
-    if (p.splits > 1) p.epoch = next_epoch(ctx);
+    if (p.splits > 1 && !slices) p.epoch = next_epoch(ctx);
     cudaError_t e = fn(grid, ctx->stream, ta, tb, p);
     if (e != cudaSuccess) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
     count_launch();
+    if (slices) {
+        SplitSum q;
+        std::memset(&q, 0, sizeof(q));
+        q.ws = ctx->scratch;
+        q.splits = slices;
+        q.batch = 1;
+        q.tiles_m = p.tiles_m;
+        q.tiles_n = p.tiles_n;
+        q.M = g.M;
+        q.N = g.N;
+        q.C = g.C;
+        q.ldc = g.N;
+        q.gated = g.tail;
+        e = launch_split_sum(ctx, q, true);
+        if (e != cudaSuccess) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
+        count_launch();
+    }
     std::ostringstream os;
-    os << (f32 ? "f32 " : "f16 ") << "gated " << form << " bn=" << (pair ? 256 : bn) << " splits=" << p.splits << " grid=" << grid;
+    os << (f32 ? "f32 " : "f16 ") << "gated " << form << " bn=" << (pair || slices ? 256 : bn) << " splits=" << p.splits << " grid=" << grid;
     set_last_kernel(os.str());
     return 0;
 }
