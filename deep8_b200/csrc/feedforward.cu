@@ -819,8 +819,7 @@ int gated_grad_x(d8k_ctx* ctx, int dtype, void* dx, int rows, int xc, int yc, co
     g.C = dx;
     g.ldc = xc;
     g.beta = accumulate ? 1 : 0;
-    g.ragged_k = true;
-    return run_gemm_long(ctx, g);
+    return run_gated_grad(ctx, g);
 }
 
 int gated_grad_w(d8k_ctx* ctx, int dtype, void* dw, int rows, int xc, int yc, const GatedOperands& o, int accumulate) {
@@ -835,8 +834,7 @@ int gated_grad_w(d8k_ctx* ctx, int dtype, void* dw, int rows, int xc, int yc, co
     g.ldc = yc;
     g.c_batch_stride = 1LL * xc * yc;
     g.beta = accumulate ? 1 : 0;
-    g.ragged_k = true;
-    return run_gemm_long(ctx, g);
+    return run_gated_grad(ctx, g);
 }
 
 int dropout(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* y, size_t n, const d8k_dropout* drop) {

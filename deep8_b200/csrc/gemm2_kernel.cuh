@@ -28,8 +28,11 @@
 
 namespace d8k {
 
-template <bool A_MN_, bool B_MN_, int STAGES_, int SUB_ = 2, bool GATED_ = false, bool SPLIT_ = false>
+template <bool A_MN_, bool B_MN_, int STAGES_, int SUB_ = 2, bool GATED_ = false, bool SPLIT_ = false, bool STORE8_ = false>
 struct Gemm2Cfg {
+    // STORE8: nothing but a store or an accumulating store, by eight epilogue warps: a short contraction's tile is over before four warps
+    // have stored the one before (300 rows, two 4096 x 4096 gradients: 54 us with four warps).
+    static constexpr bool STORE8 = STORE8_;
     // SPLIT: a work item is a tile and one of p.splits slices of the contraction (p.kb_per_split stages each); the epilogue stores the fp32
     // accumulator as it is, and split_sum_kernel adds the slices.
     static constexpr bool SPLIT = SPLIT_;
@@ -49,12 +52,12 @@ struct Gemm2Cfg {
     static constexpr int TMEM_COLS = 512;        // two accumulator buffers of 256 columns
     // GATED: eight epilogue warps (0-3 and 6-9), two for each quarter of the accumulator's rows, each half of the columns: the activation
     // makes the epilogue several times longer than a plain store, and with four warps it outlasted a K = 4096 tile's main loop
-    static constexpr int EPI_WARPS = GATED && !SPLIT ? 8 : 4, PRODUCER_WARP = 4, MMA_WARP = 5;
+    static constexpr int EPI_WARPS = (GATED && !SPLIT) || STORE8 ? 8 : 4, PRODUCER_WARP = 4, MMA_WARP = 5;
     static constexpr int THREADS = 32 * (EPI_WARPS + 2);
     static constexpr int BAR_BYTES = 256;
     // epilogue staging: per epilogue warp three slots (C, E1, E2) of 32 rows x 64 bytes (32 fp16 columns)
-    // (GATED: two slots, used in turn)
-    static constexpr int SLOTS = GATED ? 2 : 3;
+    // (eight warps: two slots each, used in turn)
+    static constexpr int SLOTS = EPI_WARPS == 8 ? 2 : 3;
     static constexpr int SLOT_BYTES = 32 * 64, STAGING_BYTES = EPI_WARPS * SLOTS * SLOT_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + BAR_BYTES + STAGING_BYTES + 1024;
     static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
@@ -405,6 +408,69 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         for (int v = 0; v < 8; ++v) __stcg(reinterpret_cast<uint4*>(part + c * 32) + v, make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]));
                     }
                 }
+            } else if constexpr (Cfg::STORE8) {
+                // this warp's half of the columns, 32 at a time through the two slots in turn; the old values of an accumulating store were
+                // requested one chunk ahead, in the coalesced pattern, and cross to "one thread per row" through the other slot
+                const int c_begin = warp < 4 ? 0 : 4;
+                using V = EpiVec<OutT>;
+                OutT* const out = reinterpret_cast<OutT*>(p.C) + warp_off;
+                uint4 old[4] = {};
+                auto fetch = [&](int c) {
+                    const int col = it.n0 + c * 32;
+                    if (!p.beta || !coalesced || col + 32 > p.N) return;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (warp_row0 + 8 * i + lr < p.M)
+                            old[i] = *reinterpret_cast<const uint4*>(out + static_cast<long long>(8 * i + lr) * p.ldc + col + lc * 8);
+                };
+                fetch(c_begin);
+#pragma unroll 1
+                for (int c = c_begin; c < c_begin + 4; ++c) {
+                    uint32_t r[32];
+                    const uint32_t slot = staging + (c & 1) * Cfg::SLOT_BYTES, other = staging + (~c & 1) * Cfg::SLOT_BYTES;
+                    const int col0 = it.n0 + c * 32;
+                    __syncwarp();
+                    ptx::tmem_ld_32x32(taddr + c * 32, r);
+                    ptx::tmem_ld_wait();
+                    if (col0 >= p.N) continue;
+                    float v[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+                    if (coalesced && col0 + 32 <= p.N) {
+                        if (p.beta) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) st_shared_v4(other + slot_off(8 * i + lr, lc), old[i]);
+                            if (c + 1 < c_begin + 4) fetch(c + 1);
+                            __syncwarp();
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                float o[8];
+                                V::unpack(ptx::ld_shared_v4(other + slot_off(lane, k)), o);
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) v[8 * k + i] += o[i];
+                            }
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) st_shared_v4(slot + slot_off(lane, k), V::pack(v + 8 * k));
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (warp_row0 + 8 * i + lr < p.M)
+                                *reinterpret_cast<uint4*>(out + static_cast<long long>(8 * i + lr) * p.ldc + col0 + lc * 8) =
+                                    ptx::ld_shared_v4(slot + slot_off(8 * i + lr, lc));
+                    } else if (p.beta) {
+                        if (row < p.M) store_row_chunk_epi<OutT, 0>(p, crow, col0, v);
+                    } else {  // rows that start anywhere, or end inside these columns: one row per store, a column per lane
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) st_shared_v4(slot + slot_off(lane, k), V::pack(v + 8 * k));
+                        __syncwarp();
+#pragma unroll 4
+                        for (int rr = 0; rr < 32; ++rr)
+                            if (warp_row0 + rr < p.M && col0 + lane < p.N)
+                                out[static_cast<long long>(rr) * p.ldc + col0 + lane] = ld_shared_half(slot + slot_off(rr, lane >> 3) + 2 * (lane & 7));
+                    }
+                }
             } else if constexpr (Cfg::GATED) {
                 // 32 columns of both projections at a time; the projections (when kept) and then h cross to whole row segments through
                 // the warp's two staging slots
@@ -487,7 +553,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                 }
             }
 #pragma unroll 1
-            for (int c = 0; c < (Cfg::GATED || Cfg::SPLIT ? 0 : 256 / 32); ++c) {
+            for (int c = 0; c < (Cfg::GATED || Cfg::SPLIT || Cfg::STORE8 ? 0 : 256 / 32); ++c) {
                 uint32_t r[32];
                 __syncwarp();
                 ptx::tmem_ld_32x32(taddr + c * 32, r);

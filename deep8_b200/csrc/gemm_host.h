@@ -64,7 +64,6 @@ struct GemmProblem {
     float epi_a = 0.f, epi_b = 0.f;
     void* E1 = nullptr;
     void* E2 = nullptr;
-    bool ragged_k = false;   // the paired kernel may also take a contraction that ends inside a k-block (see make_plan)
     int force_splits = 0;    // > 0: this many splits (bounded by the k-block count and the scratch) instead of the plan's own choice
     int ticket_base = 0;     // first of the context's tickets this launch uses (grouped launches give every contraction its own range)
     bool ws_strict = false;  // split within ws / ws_bytes, never in the context's own scratch (run_gemm_group carves that up itself)
@@ -148,8 +147,8 @@ struct PreparedGemm {
 int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture = nullptr);
 // The gated pair of products as one launch; every extent at least 1, every pointer checked by the caller
 int run_gated(Ctx* ctx, const GatedProblem& g);
-// run_gemm, or the split paired kernel where that is the faster one: fp16 products with a long contraction and few output tiles
-int run_gemm_long(Ctx* ctx, const GemmProblem& g);
+// The gated block's gradient products: run_gemm, or for fp16 the paired kernel in the form that is the fastest for the problem
+int run_gated_grad(Ctx* ctx, const GemmProblem& g);
 // The contractions of one operator (the residue classes of a strided convolution): ONE launch whose work items are all of
 // theirs when the context has a group buffer and every part runs the same one-CTA-per-SM kernel, otherwise one launch each.
 int run_gemm_group(Ctx* ctx, std::vector<GemmProblem>& parts);
@@ -172,9 +171,11 @@ GemmLaunchFn lookup_f16_gated(int bn);
 GemmLaunchFn lookup_f32_gated(int mode);
 GemmLaunchFn lookup_gated_gather(bool f32);  // loader warps: 128 columns fp16, 64 fp32
 GemmLaunchFn lookup_f16_gated_pair();
-// the same and the plain paired kernel on slices of the contraction (Gemm2Cfg::SPLIT)
+// the same and the plain paired kernel on slices of the contraction (Gemm2Cfg::SPLIT), and the latter with eight storing warps (STORE8); both
+// operands K-major, or both MN-major
 GemmLaunchFn lookup_f16_gated_pair_split();
-GemmLaunchFn lookup_f16_pair_split(bool a_mn, bool b_mn);
+GemmLaunchFn lookup_f16_pair_split(bool mn);
+GemmLaunchFn lookup_f16_pair_store(bool mn);
 // paired-CTA kernel: the first argument of the launch function is the number of CTA pairs
 GemmLaunchFn lookup_f16_pair(bool a_mn, bool b_mn);
 

@@ -1,5 +1,5 @@
-// Instantiations of the paired-CTA fp16 kernel for the gated feed-forward block: the gated product (256 x 128 outputs per pair), and split
-// contractions - the gated product's and its gradients' - whose slices split_sum_kernel adds.
+// Instantiations of the paired-CTA fp16 kernel for the gated feed-forward block: the gated product (256 x 128 outputs per pair), its gradients'
+// products with eight storing warps, and split contractions of both whose slices split_sum_kernel adds.
 #include "gemm2_kernel.cuh"
 #include "gemm_host.h"
 
@@ -9,11 +9,14 @@ GemmLaunchFn lookup_f16_gated_pair() { return launch_pair_cfg<Gemm2Cfg<false, tr
 
 GemmLaunchFn lookup_f16_gated_pair_split() { return launch_pair_cfg<Gemm2Cfg<false, true, 3, 2, true, true>>; }
 
-GemmLaunchFn lookup_f16_pair_split(bool a_mn, bool b_mn) {
-    if (!a_mn && !b_mn) return launch_pair_cfg<Gemm2Cfg<false, false, 3, 2, false, true>>;
-    if (!a_mn && b_mn) return launch_pair_cfg<Gemm2Cfg<false, true, 3, 2, false, true>>;
-    if (a_mn && !b_mn) return launch_pair_cfg<Gemm2Cfg<true, false, 3, 2, false, true>>;
-    return launch_pair_cfg<Gemm2Cfg<true, true, 3, 2, false, true>>;
+// the gradient of x multiplies two K-major operands, the gradient of w two MN-major ones
+GemmLaunchFn lookup_f16_pair_split(bool mn) {
+    if (mn) return launch_pair_cfg<Gemm2Cfg<true, true, 3, 2, false, true>>;
+    return launch_pair_cfg<Gemm2Cfg<false, false, 3, 2, false, true>>;
+}
+GemmLaunchFn lookup_f16_pair_store(bool mn) {
+    if (mn) return launch_pair_cfg<Gemm2Cfg<true, true, 3, 2, false, false, true>>;
+    return launch_pair_cfg<Gemm2Cfg<false, false, 3, 2, false, false, true>>;
 }
 
 // ------------------------------------------------------------------------------------------------ the sum of a split product's slices

@@ -353,10 +353,7 @@ Plan make_plan(const Ctx* ctx, const GemmProblem& g, size_t scratch_limit) {
     // CTA pairs on 256 x 256 tiles once the output alone fills the machine (74 pairs) and nothing is split
     int tiles256 = g.batch * ((g.M + 255) / 256) * ((g.N + 255) / 256);
     pl.pair = pl.tma && pl.a_tma == kTmaTiled && pl.b_tma == kTmaTiled && !g.out.rows_on && !g.out.cols_on && pl.bn == 256 && pl.splits == 1 && (tiles256 * 2 >= ctx->num_sms || pair_early(ctx, g) || env_int("D8K_PAIR", 1) == 2) && env_int("D8K_PAIR", 1) != 0 &&
-              // whole 64-element groups of each stored row, or rows padded to them.  An MN-major operand's k are rows, which end
-              // anywhere (what a box holds beyond is zeros); only ragged_k problems use that, the others keep the kernel they had
-              (g.K % 64 == 0 || (g.ragged_k && (g.a.mn || g.a.padded) && (g.b.mn || g.b.padded))) &&
-              (!g.a.mn || g.M % 64 == 0 || g.a.padded) && (!g.b.mn || g.N % 64 == 0 || g.b.padded);
+              g.K % 64 == 0 && (!g.a.mn || g.M % 64 == 0) && (!g.b.mn || g.N % 64 == 0);
     if (pl.pair) {
         pl.tiles_m = (g.M + 255) / 256;
         pl.tiles_n = (g.N + 255) / 256;
@@ -655,49 +652,57 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
     return 0;
 }
 
-// How many slices the paired kernel should cut a contraction of `its` stages (of 128 k) into, 0 when the ordinary kernels are faster.  The model,
-// in us, from measured times: a stage of a 256 x 256 tile 0.76, a launch with its fill and drain 6; the sum's launch 3 and its reads at 3 TB/s; a
-// k-block of 64 on the one-CTA kernel's 128 x 128 tile 0.5, whatever it multiplies.  `tiles` counts 256 x 256 tiles, `singles` the
-// one-CTA kernel's.
-static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int its, bool pair_fits_unsplit) {
+// How the gated block's fp16 products run: 0 on the one-CTA kernel, 1 on the paired kernel, more on the paired kernel in that many slices.
+// A model in us, from measured times.  Paired: a stage (128 k) of a 256 x 256 tile 0.76, but a tile not less than `store`, its epilogue; one-CTA: a
+// k-block of 64 on a 128 x 128 tile 0.5, whatever it multiplies, a tile not less than 2.5.  6 for a launch with its fill and drain; for slices 3 for the
+// sum's launch and its reads at 3 TB/s.  `tiles` counts 256 x 256 tiles, `singles` the one-CTA kernel's, `its` stages.
+static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int its, double store) {
     const int pairs = ctx->num_sms / 2;
-    const double unsplit = (tiles + pairs - 1) / pairs * its * 0.76 + 6;
+    auto rounds = [](long long work, int at_once) { return static_cast<double>((work + at_once - 1) / at_once); };
+    auto longer = [](double a, double b) { return a > b ? a : b; };
     // the one-CTA kernel splits, too, when its tiles leave half of the SMs idle: at least 24 k-blocks each
-    double single_kb = 2.0 * its, extra = 0;
+    double kb = 2.0 * its, extra = 0;
     if (singles * 2 <= ctx->num_sms) {
         long long s = ctx->num_sms / singles;
         if (s > its / 12) s = its / 12;
         if (s > 1) {
-            single_kb /= s;
+            kb /= s;
             extra = 4;
         }
     }
-    double best = (singles + ctx->num_sms - 1) / ctx->num_sms * single_kb * 0.5 + 6 + extra;
-    if (pair_fits_unsplit && unsplit < best) best = unsplit;
-    int slices = 0;
-    for (int s = 1; s <= its && s <= 32; ++s) {
+    double best = rounds(singles, ctx->num_sms) * longer(kb * 0.5, 2.5) + 6 + extra;
+    int choice = 0;
+    const double unsplit = rounds(tiles, pairs) * longer(its * 0.76, store) + 6;
+    if (unsplit < best) {
+        best = unsplit;
+        choice = 1;
+    }
+    for (int s = 2; s <= its && s <= 32; ++s) {
         const int per = (its + s - 1) / s;
         if ((its + per - 1) / per != s) continue;
         const double bytes = static_cast<double>(tiles) * s * 65536 * 4;
-        if (bytes > static_cast<double>(ctx->scratch_bytes)) break;
-        const double t = (tiles * s + pairs - 1) / pairs * per * 0.76 + 6 + 3 + bytes / 3e6;
+        if (bytes > static_cast<double>(ctx->scratch_bytes) || tiles * s >= (1LL << 30)) break;
+        const double t = rounds(tiles * s, pairs) * longer(per * 0.76, store) + 6 + 3 + bytes / 3e6;
         if (t < best) {
             best = t;
-            slices = s;
+            choice = s;
         }
     }
-    return slices;
+    return choice;
 }
 
-int run_gemm_long(Ctx* ctx, const GemmProblem& g) {
-    const bool whole = (g.K % 64 == 0 || ((g.a.mn || g.a.padded) && (g.b.mn || g.b.padded))) && (!g.a.mn || g.M % 64 == 0 || g.a.padded) &&
-                       (!g.b.mn || g.N % 64 == 0 || g.b.padded);
-    if (g.dtype != 0 || !whole || !tma_ok(g.a, 2) || !tma_ok(g.b, 2) || encode_tiled() == nullptr || !env_int("D8K_PAIR", 1) || env_int("D8K_FORCE_GATHER", 0))
-        return run_gemm(ctx, g);
+int run_gated_grad(Ctx* ctx, const GemmProblem& g) {
+    // Whole 64-element groups of each stored row, or rows padded to them.  An MN-major operand's k are rows, which end anywhere (what a box
+    // holds beyond them is zeros).
+    const bool mn = g.a.mn;
+    const bool whole = mn ? (g.M % 64 == 0 || g.a.padded) && (g.N % 64 == 0 || g.b.padded) : g.K % 64 == 0 || (g.a.padded && g.b.padded);
     const long long tiles_m = (g.M + 255LL) / 256, tiles_n = (g.N + 255LL) / 256, tiles = g.batch * tiles_m * tiles_n;
+    if (g.dtype != 0 || g.a.mn != g.b.mn || !whole || !tma_ok(g.a, 2) || !tma_ok(g.b, 2) || encode_tiled() == nullptr || tiles >= (1LL << 30) ||
+        !env_int("D8K_PAIR", 1) || env_int("D8K_FORCE_GATHER", 0))
+        return run_gemm(ctx, g);
     const long long singles = static_cast<long long>(g.batch) * ((g.M + 127LL) / 128) * ((g.N + 127LL) / 128);
     const int num_kb = (g.K + 63) / 64, its = g.kbatch * ((num_kb + 1) / 2);
-    const int slices = tiles > 4 * ctx->num_sms ? 0 : pair_slices(ctx, tiles, singles, its, tiles * 2 >= ctx->num_sms);
+    const int slices = pair_slices(ctx, tiles, singles, its, 3.0);
     if (slices == 0) return run_gemm(ctx, g);
     GemmParams p;
     std::memset(&p, 0, sizeof(p));
@@ -710,7 +715,16 @@ int run_gemm_long(Ctx* ctx, const GemmProblem& g) {
     p.tiles_m = static_cast<int>(tiles_m);
     p.tiles_n = static_cast<int>(tiles_n);
     p.raster_group = 16;
+    if (slices == 1) {
+        const Raster r = pick_raster(g.M, g.N, static_cast<long long>(g.K) * g.kbatch, p.tiles_m, p.tiles_n, ctx->num_sms / 2);
+        p.raster_group = r.group;
+        p.raster_n = r.along_n;
+    }
     p.total_work = static_cast<int>(tiles) * slices;
+    p.beta = g.beta;
+    p.C = g.C;
+    p.ldc = g.ldc;
+    p.c_batch_stride = g.c_batch_stride;
     p.ws = ctx->scratch;
     p.status = ctx->status;
     p.a_batch_mod = g.a.batch_count;
@@ -718,27 +732,29 @@ int run_gemm_long(Ctx* ctx, const GemmProblem& g) {
     CUtensorMap ta, tb;
     std::memset(&ta, 0, sizeof(ta));
     std::memset(&tb, 0, sizeof(tb));
-    if (!make_pair_map(&ta, g.a, g.M, g.K) || !make_pair_map(&tb, g.b, g.N, g.K)) return fail(2, "gemm: cuTensorMapEncodeTiled (4-D) failed");
+    if (!make_pair_map(&ta, g.a, g.M, g.K) || !make_pair_map(&tb, g.b, g.N, g.K)) return fail(2, "gated: cuTensorMapEncodeTiled (4-D) failed");
     const int pairs = p.total_work < ctx->num_sms / 2 ? p.total_work : ctx->num_sms / 2;
-    cudaError_t e = lookup_f16_pair_split(g.a.mn, g.b.mn)(pairs, ctx->stream, ta, tb, p);
-    if (e != cudaSuccess) return fail(2, std::string("gemm: launch failed: ") + cudaGetErrorString(e));
+    cudaError_t e = (slices > 1 ? lookup_f16_pair_split(mn) : lookup_f16_pair_store(mn))(pairs, ctx->stream, ta, tb, p);
+    if (e != cudaSuccess) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
     count_launch();
-    SplitSum q;
-    std::memset(&q, 0, sizeof(q));
-    q.ws = ctx->scratch;
-    q.splits = slices;
-    q.batch = g.batch;
-    q.tiles_m = p.tiles_m;
-    q.tiles_n = p.tiles_n;
-    q.M = g.M;
-    q.N = g.N;
-    q.C = g.C;
-    q.ldc = g.ldc;
-    q.c_batch_stride = g.c_batch_stride;
-    q.beta = g.beta;
-    e = launch_split_sum(ctx, q, false);
-    if (e != cudaSuccess) return fail(2, std::string("gemm: launch failed: ") + cudaGetErrorString(e));
-    count_launch();
+    if (slices > 1) {
+        SplitSum q;
+        std::memset(&q, 0, sizeof(q));
+        q.ws = ctx->scratch;
+        q.splits = slices;
+        q.batch = g.batch;
+        q.tiles_m = p.tiles_m;
+        q.tiles_n = p.tiles_n;
+        q.M = g.M;
+        q.N = g.N;
+        q.C = g.C;
+        q.ldc = g.ldc;
+        q.c_batch_stride = g.c_batch_stride;
+        q.beta = g.beta;
+        e = launch_split_sum(ctx, q, false);
+        if (e != cudaSuccess) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
+        count_launch();
+    }
     std::ostringstream os;
     os << "f16 pair slices=" << slices << " grid=" << pairs;
     set_last_kernel(os.str());
@@ -839,14 +855,13 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     const bool tma = can_tma && tma_ok(a, esize) && tma_ok(b, esize);
     if (tma && !f32 && g.M <= 128) return run_gated_few(ctx, g, a, b);
     const long long mtiles = (g.M + kBM - 1) / kBM, ptiles = (g.M + 255LL) / 256 * ((g.N + 127) / 128);
-    // The paired kernel from half a wave of its tiles on, with a long contraction from a third of one, as in make_plan.
-    const bool pair = tma && !f32 && (g.K % 64 == 0 || a.padded) && (g.N % 64 == 0 || b.padded) && env_int("D8K_PAIR", 1) != 0 &&
-                      (ptiles * 2 >= ctx->num_sms || (g.K >= 2048 && ptiles * 3 >= ctx->num_sms));
-    // a long contraction with few tiles: slices on the paired kernel
+    // fp16: the paired kernel, whole or in slices, where the model finds it faster
     const int its = (g.K + 127) / 128;
     int slices = 0;
-    if (tma && !f32 && (g.K % 64 == 0 || a.padded) && (g.N % 64 == 0 || b.padded) && env_int("D8K_PAIR", 1) != 0 && ptiles <= 4 * ctx->num_sms)
-        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, pair);
+    if (tma && !f32 && (g.K % 64 == 0 || a.padded) && (g.N % 64 == 0 || b.padded) && env_int("D8K_PAIR", 1) != 0 && ptiles < (1LL << 30))
+        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, 5.0);
+    const bool pair = slices == 1;
+    if (pair) slices = 0;
     int bn = f32 ? 64 : 128;
     if (!f32 && tma && mtiles * ((g.N + 127) / 128) >= ctx->num_sms) bn = 256;  // wide tiles when they alone give every SM one
     const long long tiles = pair || slices ? ptiles : mtiles * ((g.N + bn / 2 - 1) / (bn / 2));
