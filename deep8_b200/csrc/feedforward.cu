@@ -215,8 +215,34 @@ __device__ __forceinline__ Pack<T, W> pack_of(const float (&f)[W]) {
     return p;
 }
 
-// Copies of row-major matrices with their rows padded by zeros to whole 128-byte pieces, so that TMA can read what starts anywhere:
-// one 16-byte store per step, its elements loaded one by one.
+// 16 bytes from an address that is a multiple of the element size only: the two aligned pieces it touches, shifted together.  Both pieces must
+// be readable.
+template <int ESIZE>
+__device__ __forceinline__ uint4 load_shifted(const char* p) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uint4* q = reinterpret_cast<const uint4*>(at & ~static_cast<uintptr_t>(15));
+    const uint4 a = __ldg(q);
+    const unsigned shift = static_cast<unsigned>(at & 15);
+    if (shift == 0) return a;
+    const uint4 b = __ldg(q + 1);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (shift & 8) {
+#pragma unroll
+        for (int k = 0; k < 6; ++k) w[k] = w[k + 2];
+    }
+    if (shift & 4) {
+#pragma unroll
+        for (int k = 0; k < 5; ++k) w[k] = w[k + 1];
+    }
+    if (ESIZE == 2 && (shift & 2)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Copies of row-major matrices with their rows padded by zeros to whole 128-byte pieces, so that TMA can read what starts anywhere: a
+// 16-byte store per step from shifted 16-byte loads; a row's last piece, and what would touch memory around the matrix, element by element.
 struct PadJobs {
     PadJob job[2];
 };
@@ -228,13 +254,19 @@ __global__ void __launch_bounds__(256) pad_kernel(PadJobs jobs, int count) {
         T* dst = static_cast<T*>(jobs.job[q].dst);
         const int cols = jobs.job[q].cols, packs = jobs.job[q].pitch / W;
         const size_t total = static_cast<size_t>(jobs.job[q].rows) * packs;
+        const uintptr_t lowest = reinterpret_cast<uintptr_t>(src), highest = lowest + static_cast<size_t>(jobs.job[q].rows) * cols * sizeof(T);
         for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
             const size_t r = i / packs;
             const int c = static_cast<int>(i - r * packs) * W;
             const T* from = src + r * cols + c;
+            const uintptr_t piece = reinterpret_cast<uintptr_t>(from) & ~static_cast<uintptr_t>(15);
             Pack<T, W> v;
+            if (c + W <= cols && piece >= lowest && piece + 32 <= highest) {
+                *reinterpret_cast<uint4*>(&v) = load_shifted<sizeof(T)>(reinterpret_cast<const char*>(from));
+            } else {
 #pragma unroll
-            for (int k = 0; k < W; ++k) v.v[k] = c + k < cols ? from[k] : narrow<T>(0.0f);
+                for (int k = 0; k < W; ++k) v.v[k] = c + k < cols ? from[k] : narrow<T>(0.0f);
+            }
             store_pack(dst + i * W, v);
         }
     }
@@ -761,8 +793,8 @@ int gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, con
     return 0;
 }
 
-// The operands of the two gradient products: x [rows, xc], w and dpre [2, ...].  Where their rows do not start on 16-byte boundaries the
-// products read copies with padded rows (in the context's padding memory) that TMA can describe; the loader warps would fetch such rows
+// The operands of the two gradient products: x [rows, xc], w and dpre [2, ...].  Where their rows do not start on 16-byte boundaries (or are no
+// whole 128-byte pieces, see below) the products read copies with padded rows (in the context's padding memory) that TMA can describe; the loader warps would fetch such rows
 // element by element (333 x 250 x 1001 fp32: 203 us for both gradients).
 struct GatedOperands {
     HostOperand x, w, dpre;
@@ -781,7 +813,11 @@ int gated_operands(d8k_ctx* ctx, int dtype, GatedOperands* o, const void* x, con
     size_t bytes = 0, at[3] = {};
     bool wanted[3] = {};
     for (int k = 0; k < 3; ++k) {
-        wanted[k] = parts[k].o->ptr && !rows_aligned(parts[k].o->ptr, parts[k].cols, dtype);
+        // Rows of whole 128-byte pieces as well where that lets a faster kernel read them: x (a small copy) for the paired kernel or, in fp32, any TMA
+        // kernel; dpre for the same when it costs no copy, in fp32 always; w from 4096 rows on, where the product dwarfs the copy.
+        const bool whole = parts[k].cols % piece == 0;
+        const bool useful = !whole && (k == 0 || (k == 1 ? dtype == D8K_F16 && rows >= 4096 : dpre_to_come || dtype == D8K_F32));
+        wanted[k] = parts[k].o->ptr && (useful || !rows_aligned(parts[k].o->ptr, parts[k].cols, dtype));
         at[k] = bytes;
         if (wanted[k]) bytes += (static_cast<size_t>(parts[k].rows) * ((parts[k].cols + piece - 1) / piece * piece) * esize(dtype) + 255) & ~static_cast<size_t>(255);
     }

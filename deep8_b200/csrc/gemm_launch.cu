@@ -816,14 +816,24 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     b.batch_count = 2;
     b.batch_stride = static_cast<long long>(g.K) * g.N;
     const bool can_tma = encode_tiled() != nullptr && !env_int("D8K_FORCE_GATHER", 0);
-    if (can_tma && !(tma_ok(a, esize) && tma_ok(b, esize))) {
+    const long long mtiles = (g.M + kBM - 1) / kBM, ptiles = (g.M + 255LL) / 256 * ((g.N + 127) / 128);
+    const int its = (g.K + 127) / 128;
+    // fp16: the paired kernel, whole (1) or in slices, where the model finds it faster
+    int slices = 0;
+    if (can_tma && !f32 && g.M > 128 && env_int("D8K_PAIR", 1) != 0 && ptiles < (1LL << 30))
+        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, 5.0);
+    // The paired kernel reads rows of whole 128-byte pieces: x is copied with padded rows for it, w from 4096 rows on, where the product dwarfs the copy
+    bool pad_a = !tma_ok(a, esize) || (slices && g.K % bk != 0);
+    const bool pad_b = !tma_ok(b, esize) || (slices && g.N % bk != 0 && g.M >= 4096);
+    if (!pad_b && g.N % bk != 0) pad_a = !tma_ok(a, esize);  // x alone would not do
+    if (can_tma && (pad_a || pad_b)) {
         // Rows that do not start on 16-byte boundaries: copies with padded rows, read by TMA.  The loader warps fetch such rows element by
         // element (333 x 250 x 1001 fp32: 40 us).
         PadJob jobs[2];
         int count = 0;
         size_t bytes = 0;
-        auto plan = [&](HostOperand& o, long long rows, int cols) {
-            if (tma_ok(o, esize)) return;
+        auto plan = [&](HostOperand& o, bool wanted, long long rows, int cols) {
+            if (!wanted) return;
             PadJob& j = jobs[count++];
             j.src = o.ptr;
             j.rows = rows;
@@ -832,9 +842,9 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
             j.dst = reinterpret_cast<void*>(bytes);
             bytes += (static_cast<size_t>(rows) * j.pitch * esize + 255) & ~static_cast<size_t>(255);
         };
-        plan(a, g.M, g.K);
+        plan(a, pad_a, g.M, g.K);
         const bool a_copied = count == 1;
-        plan(b, 2LL * g.K, g.N);
+        plan(b, pad_b, 2LL * g.K, g.N);
         if (char* base = static_cast<char*>(pad_memory(ctx, bytes))) {
             for (int k = 0; k < count; ++k) jobs[k].dst = base + reinterpret_cast<size_t>(jobs[k].dst);
             if (cudaError_t e = launch_pad(ctx, g.dtype, jobs, count)) return fail(2, std::string("gated: launch failed: ") + cudaGetErrorString(e));
@@ -854,12 +864,7 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     }
     const bool tma = can_tma && tma_ok(a, esize) && tma_ok(b, esize);
     if (tma && !f32 && g.M <= 128) return run_gated_few(ctx, g, a, b);
-    const long long mtiles = (g.M + kBM - 1) / kBM, ptiles = (g.M + 255LL) / 256 * ((g.N + 127) / 128);
-    // fp16: the paired kernel, whole or in slices, where the model finds it faster
-    const int its = (g.K + 127) / 128;
-    int slices = 0;
-    if (tma && !f32 && (g.K % 64 == 0 || a.padded) && (g.N % 64 == 0 || b.padded) && env_int("D8K_PAIR", 1) != 0 && ptiles < (1LL << 30))
-        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, 5.0);
+    if (!tma || !(g.K % 64 == 0 || a.padded) || !(g.N % 64 == 0 || b.padded)) slices = 0;
     const bool pair = slices == 1;
     if (pair) slices = 0;
     int bn = f32 ? 64 : 128;

@@ -77,6 +77,7 @@ class Context:
     def __init__(self, device=0, scratch_bytes=0):
         self.lib = _lib.load()
         self.device = device
+        self._device = torch.device("cuda", device)
         self.stream = None  # torch.cuda.Stream given to use_stream
         h = ctypes.c_void_p()
         check(self.lib.d8k_ctx_create(device, scratch_bytes, ctypes.byref(h)))
@@ -345,16 +346,31 @@ class Context:
 
     # ------------------------------------------------------------------------------------------------ gated feed-forward block
     def _on_device(self, *ts):
-        """_same, and on this context's GPU."""
-        dt = _same(*ts)
-        if not ts[0].is_cuda or ts[0].device.index != self.device:
-            raise ValueError("the device type must be same")
-        return dt
+        """_same, and on this context's GPU (in one pass: a small call's time is its host time)."""
+        device, dtype = self._device, ts[0].dtype
+        for t in ts:
+            if t.device != device:
+                raise ValueError("the device type must be same")
+            if t.dtype != dtype:
+                raise ValueError("the data type must be same")
+            if not t.is_contiguous():
+                raise ValueError("tensors must be contiguous")
+        return _dtype_code(ts[0])
+
+    @staticmethod
+    def _like(out, like):
+        """_out for an output with the shape of `like`."""
+        if out is None:
+            return torch.empty_like(like)
+        _same(like, out)
+        if out.shape != like.shape:
+            raise ValueError("the shape is error")
+        return out
 
     def _drop_arg(self, dropout):
         if dropout is None:
             return None
-        if dropout.counter is not None and (not dropout.counter.is_cuda or dropout.counter.device.index != self.device):
+        if dropout.counter is not None and dropout.counter.device != self._device:
             raise ValueError("the device type must be same")
         return dropout.arg
 
@@ -382,11 +398,12 @@ class Context:
         dt = self._on_device(x, w) if pre is None else self._on_device(x, w, pre)
         xb, xr, xc, yc = self._gated_dims(x, w)
         act = self._activation(activation)
-        if pre is not None and tuple(pre.shape) != (2, xb * xr, yc):
+        if pre is not None and pre.shape != (2, xb * xr, yc):
             raise ValueError("the shape is error")
         drop = self._drop_arg(dropout)
         h = _out(out, (xb, xr, yc), x)
-        check(self.lib.d8k_gated_forward(self.h, dt, act, _p(x), xb, xr, xc, _p(w), yc, _p(pre), _p(h), drop))
+        check(self.lib.d8k_gated_forward(self.h, dt, act, x.data_ptr(), xb, xr, xc, w.data_ptr(), yc, pre.data_ptr() if pre is not None else None,
+                                         h.data_ptr(), drop))
         return h
 
     def gated_grad_pre(self, pre, dz, activation="silu", dpre=None, dropout=None):
@@ -432,8 +449,9 @@ class Context:
         if residual is not None and residual.shape != x.shape:
             raise ValueError("the shape is error")
         drop = self._drop_arg(dropout)
-        y = _out(out, tuple(x.shape), x)
-        check(self.lib.d8k_dropout_forward(self.h, dt, _p(x), _p(residual), _p(y), x.numel(), drop))
+        y = self._like(out, x)
+        check(self.lib.d8k_dropout_forward(self.h, dt, x.data_ptr(), residual.data_ptr() if residual is not None else None, y.data_ptr(), x.numel(),
+                                           drop))
         return y
 
     def dropout_backward(self, dx, dy, dropout, accumulate=True):
@@ -441,7 +459,7 @@ class Context:
         dt = self._on_device(dx, dy)
         if dx.shape != dy.shape:
             raise ValueError("the shape is error")
-        check(self.lib.d8k_dropout_backward(self.h, dt, _p(dx), _p(dy), dy.numel(), int(accumulate), self._drop_arg(dropout)))
+        check(self.lib.d8k_dropout_backward(self.h, dt, dx.data_ptr(), dy.data_ptr(), dy.numel(), int(accumulate), self._drop_arg(dropout)))
         return dx
 
     @staticmethod
@@ -455,23 +473,27 @@ class Context:
         """y = x * rstd * weight, rstd = 1 / sqrt(mean(x^2) + eps) over the last dimension.  rstd: optional float32 tensor with one element per
         row that receives the factors the backward pass reads; out may be x."""
         dt = self._on_device(x, weight)
-        if x.dim() < 1 or x.shape[-1] < 1 or weight.numel() != x.shape[-1]:
-            raise ValueError("the shape is error")
-        cols = x.shape[-1]
-        rows = x.numel() // cols
+        rows, cols = self._norm_dims(x, weight)
         if rstd is not None:
             self._check_rstd(rstd, rows, x)
-        y = _out(out, tuple(x.shape), x)
-        check(self.lib.d8k_rms_norm_forward(self.h, dt, _p(x), _p(weight), float(eps), _p(y), _p(rstd), rows, cols))
+        y = self._like(out, x)
+        check(self.lib.d8k_rms_norm_forward(self.h, dt, x.data_ptr(), weight.data_ptr(), float(eps), y.data_ptr(),
+                                            rstd.data_ptr() if rstd is not None else None, rows, cols))
         return y
+
+    @staticmethod
+    def _norm_dims(x, weight):
+        cols = weight.numel()
+        if x.dim() < 1 or cols < 1 or x.shape[-1] != cols:
+            raise ValueError("the shape is error")
+        return x.numel() // cols, cols
 
     def rms_norm_backward(self, x, weight, rstd, dx, dweight, dy, accumulate=True):
         """dx (+)= and dweight (+)= the gradients of rms_norm_forward for dy; dx or dweight may be None."""
         dt = self._on_device(x, weight, dy)
-        if x.dim() < 1 or x.shape[-1] < 1 or weight.numel() != x.shape[-1] or dy.shape != x.shape:
+        rows, cols = self._norm_dims(x, weight)
+        if dy.shape != x.shape:
             raise ValueError("the shape is error")
-        cols = x.shape[-1]
-        rows = x.numel() // cols
         self._check_rstd(rstd, rows, x)
         for grad, like in ((dx, x), (dweight, weight)):
             if grad is not None:
