@@ -363,8 +363,11 @@ __device__ __forceinline__ Pack<T, E> drop_pack(const Pack<T, E>& a, const Pack<
 // y = (residual +) dropout(x): `residual` is the accumulated gradient itself in the backward pass.  VEC: bases on 16-byte boundaries; the
 // last, partial pack goes element by element either way.  A launch covers at most 2^34 elements, whose counters share their high
 // word.  y may be x or residual, so nothing is declared __restrict__.
+// Bound by HBM in fp32 (8192 x 4096: 45.7 us, with a residual 64.7: 5.9 and 6.2 TB/s) and by the generator in fp16 (35.5 us, with a residual
+// 37.5: the ten rounds alone take 27 us for these 2^25 words).  The registers are kept to what lets eight (fp32: six) CTAs hide each
+// other's loads and rounds: 37.6 and 40.6 us with five.
 template <typename T, bool VEC, bool ADD>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* x, const T* residual, T* y, size_t n, uint32_t group_hi, DropSpec drop) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 6) dropout_kernel(const T* x, const T* residual, T* y, size_t n, uint32_t group_hi, DropSpec drop) {
     constexpr int E = VEC ? 16 / sizeof(T) : 4;
     const unsigned long long offset = drop_offset(drop);
     const size_t whole = n / E, stride = gridDim.x * static_cast<size_t>(blockDim.x);
