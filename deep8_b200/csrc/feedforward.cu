@@ -858,6 +858,7 @@ int gated_grad_x(d8k_ctx* ctx, int dtype, void* dx, int rows, int xc, int yc, co
     g.C = dx;
     g.ldc = xc;
     g.beta = accumulate ? 1 : 0;
+    g.precise = true;
     return run_gated_grad(ctx, g);
 }
 
@@ -873,6 +874,7 @@ int gated_grad_w(d8k_ctx* ctx, int dtype, void* dw, int rows, int xc, int yc, co
     g.ldc = yc;
     g.c_batch_stride = 1LL * xc * yc;
     g.beta = accumulate ? 1 : 0;
+    g.precise = true;
     return run_gated_grad(ctx, g);
 }
 

@@ -64,6 +64,7 @@ struct GemmProblem {
     float epi_a = 0.f, epi_b = 0.f;
     void* E1 = nullptr;
     void* E2 = nullptr;
+    bool precise = false;    // fp32 with short accumulation chains (GemmCfg::PRECISE); both operands K-major or both MN-major
     int force_splits = 0;    // > 0: this many splits (bounded by the k-block count and the scratch) instead of the plan's own choice
     int ticket_base = 0;     // first of the context's tickets this launch uses (grouped launches give every contraction its own range)
     bool ws_strict = false;  // split within ws / ws_bytes, never in the context's own scratch (run_gemm_group carves that up itself)
@@ -176,6 +177,7 @@ GemmLaunchFn lookup_f16_gated_pair();
 GemmLaunchFn lookup_f16_gated_pair_split();
 GemmLaunchFn lookup_f16_pair_split(bool mn);
 GemmLaunchFn lookup_f16_pair_store(bool mn);
+GemmLaunchFn lookup_f32_precise(bool mn, int mode);  // mode 1, 2 or 4 as in lookup_f32_dual, 0 the loader warps
 // paired-CTA kernel: the first argument of the launch function is the number of CTA pairs
 GemmLaunchFn lookup_f16_pair(bool a_mn, bool b_mn);
 

@@ -253,7 +253,7 @@ __device__ __forceinline__ long long scatter_offset(const GemmParams& p, int row
 }
 
 template <bool F32_, bool A_MN_, bool B_MN_, int BN_, int STAGES_, bool GATHER_, bool ATMEM_ = false, bool HALO_ = false, int DUAL_ = 0,
-          bool GATED_ = false>
+          bool GATED_ = false, bool PRECISE_ = GATED_>
 struct GemmCfg {
     static constexpr bool F32 = F32_, A_MN = A_MN_, B_MN = B_MN_, GATHER = GATHER_;
     static constexpr int BN = BN_, STAGES = STAGES_;
@@ -318,7 +318,14 @@ struct GemmCfg {
     // 2e-5 of the result after 1300 accumulations).  Every CHUNK_KB k-blocks the accumulator buffer is handed to the
     // epilogue warps, which add it to register accumulators with round-to-nearest, and a fresh chain starts in the
     // other buffer.  0 = one chain per work item (fp16, whose output rounding is far coarser).
-    static constexpr int CHUNK_KB = F32 ? 8 : 0;
+    static constexpr int CHUNK_KB = F32 ? (PRECISE_ ? 4 : 8) : 0;
+    // PRECISE (the gated block's products): chains of four k-blocks, and A_lo B_hi joins A_hi B_lo in the second half of the accumulator instead of
+    // the large terms in the first, which then takes one truncated addition per k-step instead of two.  Truncation always shrinks a sum, so
+    // the chains' errors do not cancel: relative to the result (in norm) 2.9e-6 with the 64 such additions of an ordinary chain, 4.2e-7 with
+    // these 16 (2.8e-7 with chains of two k-blocks); a plain fp32 product is 3e-7 to 1.6e-6 off.  Two CTAs per SM, whose one accumulator
+    // buffer each is handed over more often, take 6 to 9 % longer for it (2000 x 1024 x 4000: 239 -> 256 us; 283 with chains of two).
+    static constexpr bool PRECISE = PRECISE_;
+    static_assert(!F32 || !PRECISE || STACK, "the second half of the accumulator holds the small terms");
     static constexpr int EPI_WARPS = 4;
     // GATHER: LOADER_GROUPS groups of four loader warps take the k-blocks in turn, so one group's address arithmetic and
     // conversions overlap the other group's global-load latency (a lone group spent 4-8 us per k-block).
@@ -1168,10 +1175,10 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                             const uint32_t ta_hi = ta_run + s * Cfg::UMMA_K;
                             if constexpr (Cfg::ALO) {
                                 ptx::mma_tf32(d_tmem, da, db, idesc_wide, accumulate);    // A_hi (shared memory) [B_hi ; B_lo]
-                                ptx::mma_tf32_a_tmem(d_tmem, ta_hi, db, idesc, 1u);      // A_lo (tensor memory) B_hi
+                                ptx::mma_tf32_a_tmem(d_tmem + (Cfg::PRECISE ? BN : 0), ta_hi, db, idesc, 1u);  // A_lo (tensor memory) B_hi
                             } else if constexpr (Cfg::STACK) {
                                 ptx::mma_tf32_a_tmem(d_tmem, ta_hi, db, idesc_wide, accumulate);  // A_hi [B_hi ; B_lo]
-                                ptx::mma_tf32_a_tmem(d_tmem, ta_hi + BK, db, idesc, 1u);          // A_lo B_hi
+                                ptx::mma_tf32_a_tmem(d_tmem + (Cfg::PRECISE ? BN : 0), ta_hi + BK, db, idesc, 1u);  // A_lo B_hi
                             } else {
                                 ptx::mma_tf32_a_tmem(d_tmem, ta_hi + BK, db, idesc, accumulate);  // small terms first
                                 ptx::mma_tf32_a_tmem(d_tmem, ta_hi, db + (Cfg::B_BYTES >> 4), idesc, 1u);
@@ -1181,7 +1188,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                             const uint64_t da_lo = da + (Cfg::A_BYTES >> 4), db_lo = db + (Cfg::B_BYTES >> 4);
                             if constexpr (Cfg::STACK) {
                                 ptx::mma_tf32(d_tmem, da, db, idesc_wide, accumulate);  // A_hi [B_hi ; B_lo]
-                                ptx::mma_tf32(d_tmem, da_lo, db, idesc, 1u);           // A_lo B_hi
+                                ptx::mma_tf32(d_tmem + (Cfg::PRECISE ? BN : 0), da_lo, db, idesc, 1u);  // A_lo B_hi
                             } else {
                                 ptx::mma_tf32(d_tmem, da_lo, db, idesc, accumulate);  // small terms first
                                 ptx::mma_tf32(d_tmem, da, db_lo, idesc, 1u);

@@ -589,10 +589,10 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
             int mode = env_int("D8K_F32_DUAL", -1);
             if (mode < 0) mode = (pl.splits == 1 && p.total_work > ctx->num_sms) ? (pl.total_kb > 8 ? 2 : 1) : 4;
             if (mode == 1 || mode == 2) {
-                fn = lookup_f32_dual(g.a.mn, g.b.mn, mode);
+                fn = g.precise ? lookup_f32_precise(g.a.mn, mode) : lookup_f32_dual(g.a.mn, g.b.mn, mode);
                 dual = true;
             } else if (mode == 4) {
-                fn = lookup_f32_dual(g.a.mn, g.b.mn, mode);
+                fn = g.precise ? lookup_f32_precise(g.a.mn, mode) : lookup_f32_dual(g.a.mn, g.b.mn, mode);
                 twin = true;
             }
         }
@@ -606,7 +606,8 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
     } else {
         p.a = g.a.mn ? to_gather(g.a, g.K, g.M, esize) : to_gather(g.a, g.M, g.K, esize);
         p.b = g.b.mn ? to_gather(g.b, g.K, g.N, esize) : to_gather(g.b, g.N, g.K, esize);
-        fn = pl.f32 ? lookup_f32_gather(g.a.mn, g.b.mn, pl.bn) : lookup_f16_gather(g.a.mn, g.b.mn, pl.bn);
+        if (g.precise && pl.f32 && pl.bn == 64) fn = lookup_f32_precise(g.a.mn, 0);
+        else fn = pl.f32 ? lookup_f32_gather(g.a.mn, g.b.mn, pl.bn) : lookup_f16_gather(g.a.mn, g.b.mn, pl.bn);
     }
     if (!fn) return fail(2, "gemm: no kernel for this configuration");
     int grid = p.total_work < ctx->num_sms ? p.total_work : ctx->num_sms;
