@@ -624,6 +624,78 @@ void AXPBY(const Tensor& x, float alpha, const Tensor& y, float beta, Tensor& z)
     DEEP8_ARGUMENT_CHECK(y.raw() == z.raw(), "on this path AXPBY updates y in place (z must be y), as the trainers call it");
     d8kCheck(d8k_axpby(gpuOf(x)->kernels, d8kType(x), x.raw(), alpha, z.raw(), beta, x.size()));
 }
+// ---- a gated feed-forward block
+namespace {
+d8k_dropout maskOf(const DropoutMask& m) { return d8k_dropout{m.p, m.seed, m.offset, m.deviceOffset}; }
+void checkGated(const Tensor& x, const Tensor& w, const Tensor& y) {
+    DEEP8_ARGUMENT_CHECK(x.device() == w.device() && x.device() == y.device(), "the device type must be same");
+    DEEP8_ARGUMENT_CHECK(x.elementType == w.elementType && x.elementType == y.elementType, "the data type must be same");
+    DEEP8_ARGUMENT_CHECK(2 == w.batch() && w.row() == x.col() && y.batch() == x.batch() && y.row() == x.row() && y.col() == w.col(), "the shape is error");
+}
+// rows of the last dimension, which `weight` matches
+size_t normRows(const Tensor& x, const Tensor& weight) {
+    DEEP8_ARGUMENT_CHECK(x.device() == weight.device() && x.elementType == weight.elementType, "the device and data type must be same");
+    const size_t cols = x.dim(x.nDims() - 1);
+    DEEP8_ARGUMENT_CHECK(weight.size() == cols, "the shape is error");
+    return x.size() / cols;
+}
+}  // namespace
+void GatedProduct(const Tensor& x, const Tensor& w, Activation activation, const DropoutMask& mask, void* pre, Tensor& y) {
+    checkGated(x, w, y);
+    const d8k_dropout drop = maskOf(mask);
+    d8kCheck(d8k_gated_forward(gpuOf(x)->kernels, d8kType(x), (int)activation, x.raw(), (int)x.batch(), (int)x.row(), (int)x.col(), w.raw(), (int)w.col(), pre,
+                               y.raw(), &drop));
+}
+void GatedProductGrad(const Tensor& x, Tensor* dx, const Tensor& w, Tensor* dw, Activation activation, const DropoutMask& mask, const void* pre, void* dpre,
+                      const Tensor& dy, bool accumulateDx, bool accumulateDw) {
+    checkGated(x, w, dy);
+    DEEP8_ARGUMENT_CHECK((nullptr == dx || (dx->shape == x.shape && dx->elementType == x.elementType)) &&
+                             (nullptr == dw || (dw->shape == w.shape && dw->elementType == w.elementType)),
+                         "the shape or type is error");
+    const d8k_dropout drop = maskOf(mask);
+    d8k_ctx* kernels = gpuOf(x)->kernels;
+    const int type = d8kType(x), batch = (int)x.batch(), row = (int)x.row(), col = (int)x.col(), width = (int)w.col();
+    if (accumulateDx == accumulateDw || nullptr == dx || nullptr == dw) {
+        d8kCheck(d8k_gated_backward(kernels, type, (int)activation, x.raw(), batch, row, col, w.raw(), width, pre, dy.raw(), dpre, dx ? dx->raw() : nullptr,
+                                    dw ? dw->raw() : nullptr, (dx ? accumulateDx : accumulateDw) ? 1 : 0, &drop));
+        return;
+    }
+    d8kCheck(d8k_gated_grad_pre(kernels, type, (int)activation, pre, dy.raw(), dpre, dy.size(), &drop));
+    d8kCheck(d8k_gated_grad_x_into(kernels, type, dx->raw(), batch, row, col, w.raw(), width, dpre, accumulateDx ? 1 : 0));
+    d8kCheck(d8k_gated_grad_w_into(kernels, type, x.raw(), batch, row, col, dw->raw(), width, dpre, accumulateDw ? 1 : 0));
+}
+void Dropout(const Tensor& x, const Tensor* residual, const DropoutMask& mask, Tensor& y) {
+    DEEP8_ARGUMENT_CHECK(x.shape == y.shape && (nullptr == residual || residual->shape == x.shape), "the param shape must be same");
+    DEEP8_ARGUMENT_CHECK(x.elementType == y.elementType && (nullptr == residual || residual->elementType == x.elementType), "the param data type must be same");
+    DEEP8_ARGUMENT_CHECK(x.device() == y.device() && (nullptr == residual || residual->device() == x.device()), "the param device type must be same");
+    const d8k_dropout drop = maskOf(mask);
+    d8kCheck(d8k_dropout_forward(gpuOf(x)->kernels, d8kType(x), x.raw(), residual ? residual->raw() : nullptr, y.raw(), x.size(), &drop));
+}
+void DropoutGrad(Tensor& dx, const DropoutMask& mask, const Tensor& dy) {
+    DEEP8_ARGUMENT_CHECK(dx.shape == dy.shape && dx.elementType == dy.elementType && dx.device() == dy.device(), "the shape, type or device is error");
+    const d8k_dropout drop = maskOf(mask);
+    d8kCheck(d8k_dropout_backward(gpuOf(dx)->kernels, d8kType(dx), dx.raw(), dy.raw(), dy.size(), OverwriteGradient::active() ? 0 : 1, &drop));
+}
+void RMSNorm(const Tensor& x, const Tensor& weight, float epsilon, float* rstd, Tensor& y) {
+    DEEP8_ARGUMENT_CHECK(x.shape == y.shape && x.elementType == y.elementType && x.device() == y.device(), "the shape, type or device is error");
+    const size_t rows = normRows(x, weight);
+    d8kCheck(d8k_rms_norm_forward(gpuOf(x)->kernels, d8kType(x), x.raw(), weight.raw(), epsilon, y.raw(), rstd, rows, (int)weight.size()));
+}
+void RMSNormGrad(const Tensor& x, Tensor* dx, const Tensor& weight, Tensor* dweight, const float* rstd, const Tensor& dy, bool accumulateDx,
+                 bool accumulateDweight) {
+    DEEP8_ARGUMENT_CHECK(x.shape == dy.shape && (nullptr == dx || dx->shape == x.shape) && (nullptr == dweight || dweight->shape == weight.shape), "the shape is error");
+    const size_t rows = normRows(x, weight);
+    auto run = [&](Tensor* a, Tensor* b, bool accumulate) {
+        d8kCheck(d8k_rms_norm_backward(gpuOf(x)->kernels, d8kType(x), x.raw(), weight.raw(), rstd, a ? a->raw() : nullptr, b ? b->raw() : nullptr, dy.raw(), rows,
+                                       (int)weight.size(), accumulate ? 1 : 0));
+    };
+    if (accumulateDx == accumulateDweight || nullptr == dx || nullptr == dweight) {
+        run(dx, dweight, dx ? accumulateDx : accumulateDweight);
+    } else {
+        run(dx, nullptr, accumulateDx);
+        run(nullptr, dweight, accumulateDweight);
+    }
+}
 void Constant(Tensor& x, float scalar) {
     DEEP8_ARGUMENT_CHECK(0.f == scalar, "only the constant 0 is supported on this path");
     d8kCheck(d8k_zero(gpuOf(x)->kernels, x.raw(), x.byteCount()));
@@ -923,6 +995,105 @@ void Linear::forward(const std::vector<const Tensor*>& in, Tensor* out) { Math::
 void Linear::backward(const std::vector<const Tensor*>& in, const Tensor* out, const Tensor* dOut, size_t index, Tensor* dIn) {
     DEEP8_ARGUMENT_CHECK(0 == index, "the index is error");
     Math::LinearGrad(*in[0], *dIn, a, b, *out, *dOut);
+}
+
+// ---- nodes of a gated feed-forward block
+namespace {
+// The output of a node in the backward walk, its gradient made real (Function::backward's rule for a gradient nothing has contributed to)
+Variable* outputWithGradient(Function* f) {
+    DEEP8_ARGUMENT_CHECK(1 == f->outputs.size(), "the output size must be 1");
+    auto out = static_cast<Variable*>(f->outputs.first());
+    if (out->updateGradient && !out->gradientTouched) {
+        out->zeroGradient();
+        out->gradientTouched = true;
+    }
+    return out;
+}
+}  // namespace
+
+GatedProduct::GatedProduct(std::vector<Node*>& in, Activation a, const DropoutMask& m) : Function(in), activation(a), mask(m) {
+    functionType = FunctionType::GatedProduct;
+    DEEP8_ARGUMENT_CHECK(2 == this->inputs.size(), "the GatedProduct Function needs 2 inputs");
+}
+GatedProduct::~GatedProduct() {
+    if (nullptr != pre) device->free(pre);
+}
+Shape GatedProduct::checkShape(std::vector<Shape>& s) {
+    DEEP8_ARGUMENT_CHECK(2 == s.size(), "the input count must be 2");
+    DEEP8_ARGUMENT_CHECK(2 == s[0].nDims && 2 == s[1].nDims && 2 == s[1].batch, "the weights of a gated product are a batch of two matrices");
+    DEEP8_ARGUMENT_CHECK(s[0].col() == s[1].row(), "the col of input1 must same to the row of input2");
+    return Shape(s[0].batch, {s[0].row(), s[1].col()});
+}
+void GatedProduct::forward(const std::vector<const Tensor*>& in, Tensor* out) {
+    bool keep = false;
+    for (auto item : inputs) keep = keep || static_cast<Variable*>(item)->updateGradient;
+    if (keep && nullptr == pre) {
+        device = out->device();
+        pre = device->malloc(2 * out->byteCount());
+    }
+    Math::GatedProduct(*in[0], *in[1], activation, mask, pre, *out);
+}
+void GatedProduct::backward() {
+    auto out = outputWithGradient(this);
+    auto x = static_cast<Variable*>(inputs[0]), w = static_cast<Variable*>(inputs[1]);
+    if (!x->updateGradient && !w->updateGradient) return;
+    DEEP8_ARGUMENT_CHECK(nullptr != pre && x != w, "the products of the forward pass were not kept");
+    void* dpre = device->malloc(2 * out->value.byteCount());
+    try {
+        Math::GatedProductGrad(x->value, x->updateGradient ? &x->gradient : nullptr, w->value, w->updateGradient ? &w->gradient : nullptr, activation, mask, pre,
+                               dpre, out->gradient, x->gradientTouched, w->gradientTouched);
+    } catch (...) {
+        device->free(dpre);
+        throw;
+    }
+    device->free(dpre);  // safe: one stream, host-side bookkeeping
+    if (x->updateGradient) x->gradientTouched = true;
+    if (w->updateGradient) w->gradientTouched = true;
+}
+
+Dropout::Dropout(std::vector<Node*>& in, const DropoutMask& m) : Function(in), mask(m) {
+    functionType = FunctionType::Dropout;
+    DEEP8_ARGUMENT_CHECK(1 == this->inputs.size() || 2 == this->inputs.size(), "the Dropout Function needs 1 or 2 inputs");
+}
+Shape Dropout::checkShape(std::vector<Shape>& s) {
+    DEEP8_ARGUMENT_CHECK(1 == s.size() || (2 == s.size() && s[0] == s[1]), "the residual must have the shape of the input");
+    return s[0];
+}
+void Dropout::forward(const std::vector<const Tensor*>& in, Tensor* out) { Math::Dropout(*in[0], 2 == in.size() ? in[1] : nullptr, mask, *out); }
+void Dropout::backward(const std::vector<const Tensor*>& in, const Tensor* out, const Tensor* dOut, size_t index, Tensor* dIn) {
+    if (0 == index) Math::DropoutGrad(*dIn, mask, *dOut);
+    else if (1 == index) Math::AddGradX(*in[1], *dIn, *in[0], *out, *dOut);
+    else DEEP8_RUNTIME_ERROR("the index is error");
+}
+
+RMSNorm::RMSNorm(std::vector<Node*>& in, float e) : Function(in), epsilon(e) {
+    functionType = FunctionType::RMSNorm;
+    DEEP8_ARGUMENT_CHECK(2 == this->inputs.size(), "the RMSNorm Function needs 2 inputs");
+}
+RMSNorm::~RMSNorm() {
+    if (nullptr != rstd) device->free(rstd);
+}
+Shape RMSNorm::checkShape(std::vector<Shape>& s) {
+    DEEP8_ARGUMENT_CHECK(2 == s.size(), "the input count must be 2");
+    DEEP8_ARGUMENT_CHECK(s[1].size() == s[0].dim(s[0].nDims - 1), "the weight must match the last dimension");
+    return s[0];
+}
+void RMSNorm::forward(const std::vector<const Tensor*>& in, Tensor* out) {
+    if (nullptr == rstd) {
+        device = out->device();
+        rstd = static_cast<float*>(device->malloc(in[0]->size() / in[1]->size() * sizeof(float)));
+    }
+    Math::RMSNorm(*in[0], *in[1], epsilon, rstd, *out);
+}
+void RMSNorm::backward() {
+    auto out = outputWithGradient(this);
+    auto x = static_cast<Variable*>(inputs[0]), w = static_cast<Variable*>(inputs[1]);
+    if (!x->updateGradient && !w->updateGradient) return;
+    DEEP8_ARGUMENT_CHECK(nullptr != rstd && x != w, "the norm has not run");
+    Math::RMSNormGrad(x->value, x->updateGradient ? &x->gradient : nullptr, w->value, w->updateGradient ? &w->gradient : nullptr, rstd, out->gradient,
+                      x->gradientTouched, w->gradientTouched);
+    if (x->updateGradient) x->gradientTouched = true;
+    if (w->updateGradient) w->gradientTouched = true;
 }
 
 // ================================================================================================ executors
@@ -1285,6 +1456,27 @@ Variable& Variable::linear(float a, float b) {
     return *executor->addFunction(new Linear(in, a, b));
 }
 Variable& linear(Variable& x, float a, float b) { return x.linear(a, b); }
+
+Variable& Variable::gatedProduct(Variable& w, Activation activation, const DropoutMask& mask) {
+    std::vector<Node*> in = {this, &w};
+    return *executor->addFunction(new GatedProduct(in, activation, mask));
+}
+Variable& Variable::dropout(const DropoutMask& mask) {
+    std::vector<Node*> in = {this};
+    return *executor->addFunction(new Dropout(in, mask));
+}
+Variable& Variable::dropout(const DropoutMask& mask, Variable& residual) {
+    std::vector<Node*> in = {this, &residual};
+    return *executor->addFunction(new Dropout(in, mask));
+}
+Variable& Variable::rmsNorm(Variable& weight, float epsilon) {
+    std::vector<Node*> in = {this, &weight};
+    return *executor->addFunction(new RMSNorm(in, epsilon));
+}
+Variable& gatedProduct(Variable& x, Variable& w, Activation activation, const DropoutMask& mask) { return x.gatedProduct(w, activation, mask); }
+Variable& dropout(Variable& x, const DropoutMask& mask) { return x.dropout(mask); }
+Variable& dropout(Variable& x, const DropoutMask& mask, Variable& residual) { return x.dropout(mask, residual); }
+Variable& rmsNorm(Variable& x, Variable& weight, float epsilon) { return x.rmsNorm(weight, epsilon); }
 
 Variable& Variable::add(Variable& y) {
     std::vector<Node*> in = {this, &y};

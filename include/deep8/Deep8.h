@@ -10,6 +10,7 @@
 //   Executor, EagerExecutor         deep8/include/model/Executor.h, EagerExecutor.h
 //   Math::*                          deep8/include/math/{MatrixMultiply,Conv2d,DeConv2d,ReLu}.h
 //   parameter(), operator*, conv2d(), deConv2d(), relu(), backward()   deep8/include/model/Net.h
+//   GatedProduct, Dropout, RMSNorm  (no counterpart there: the nodes of a gated feed-forward block)
 //
 // There is no CPU device here: every tensor lives on a GPU and every operator runs the sm_100a kernels.
 #ifndef DEEP8_B200_DEEP8_H
@@ -262,6 +263,16 @@ public:
 };
 
 // ------------------------------------------------------------------------------------------------ math (GPU only)
+// ---- a gated feed-forward block (additions; d8k.h describes the operators)
+enum class Activation { SiLu = 0, Gelu = 1, GeluTanh = 2, ReLu = 3, Sigmoid = 4 };
+// A dropout mask, which is computed wherever it is needed and never stored: the same values give the same mask, so calls that are to
+// differ take different offsets.  p == 0 drops nothing.  deviceOffset: optional 64-bit word in device memory that is added to offset.
+struct DropoutMask {
+    double p = 0;
+    unsigned long long seed = 0, offset = 0;
+    const unsigned long long* deviceOffset = nullptr;
+};
+
 namespace Math {
 DEEP8_API void MatrixMultiply(const Tensor& x, const Tensor& y, Tensor& z);
 DEEP8_API void MatrixMultiplyGPU(const Tensor& x, const Tensor& y, Tensor& z);
@@ -331,6 +342,19 @@ DEEP8_API void AddGradX(const Tensor& x, Tensor& dx, const Tensor& y, const Tens
 DEEP8_API void AddGradY(const Tensor& x, const Tensor& y, Tensor& dy, const Tensor& z, const Tensor& dz);
 // Math::AXPBY (deep8/src/math/AXPBY.cpp:6-20) with z == y, which is how every trainer calls it: y = x * alpha + y * beta
 DEEP8_API void AXPBY(const Tensor& x, float alpha, const Tensor& y, float beta, Tensor& z);
+
+// y = dropout(activation(x * w[0]) * (x * w[1])), w a batch of two; pre (device memory for twice y's elements, or null) receives both products
+DEEP8_API void GatedProduct(const Tensor& x, const Tensor& w, Activation activation, const DropoutMask& mask, void* pre, Tensor& y);
+// From pre: the gradient of both products into dpre (as large as pre, may be pre), then dx and dw where not null, added or overwritten
+DEEP8_API void GatedProductGrad(const Tensor& x, Tensor* dx, const Tensor& w, Tensor* dw, Activation activation, const DropoutMask& mask,
+                                const void* pre, void* dpre, const Tensor& dy, bool accumulateDx, bool accumulateDw);
+// y = (residual +) dropout(x); dx (+)= dropout(dy) with the same mask (overwriting under an OverwriteGradient guard)
+DEEP8_API void Dropout(const Tensor& x, const Tensor* residual, const DropoutMask& mask, Tensor& y);
+DEEP8_API void DropoutGrad(Tensor& dx, const DropoutMask& mask, const Tensor& dy);
+// y = x * rstd * weight, rstd = 1 / sqrt(mean(x^2) + epsilon) over the last dimension; rstd: device memory for a float per row, or null
+DEEP8_API void RMSNorm(const Tensor& x, const Tensor& weight, float epsilon, float* rstd, Tensor& y);
+DEEP8_API void RMSNormGrad(const Tensor& x, Tensor* dx, const Tensor& weight, Tensor* dweight, const float* rstd, const Tensor& dy,
+                           bool accumulateDx, bool accumulateDweight);
 }  // namespace Math
 
 // ------------------------------------------------------------------------------------------------ graph nodes
@@ -409,9 +433,14 @@ public:
     Variable& relu();
     Variable& add(Variable& y);
     Variable& linear(float a = 1, float b = 0);
+    // additions
+    Variable& gatedProduct(Variable& w, Activation activation = Activation::SiLu, const DropoutMask& mask = DropoutMask());
+    Variable& dropout(const DropoutMask& mask);
+    Variable& dropout(const DropoutMask& mask, Variable& residual);
+    Variable& rmsNorm(Variable& weight, float epsilon = 1e-6f);
 };
 
-enum class FunctionType { Unkown = 0, Add, Conv2d, DeConv2d, Linear, MatrixMultiply, ReLu };
+enum class FunctionType { Unkown = 0, Add, Conv2d, DeConv2d, Linear, MatrixMultiply, ReLu, GatedProduct, Dropout, RMSNorm };
 
 class DEEP8_API Function : public Node {
 protected:
@@ -497,6 +526,54 @@ public:
     void forward(const std::vector<const Tensor*>& inputs, Tensor* output) override;
     void backward(const std::vector<const Tensor*>& inputs, const Tensor* output, const Tensor* outputGradient, size_t index,
                   Tensor* iGradient) override;
+};
+
+// ---- nodes of a gated feed-forward block (additions): Math::GatedProduct, Math::Dropout and Math::RMSNorm
+class DEEP8_API GatedProduct : public Function {
+public:
+    Activation activation;
+    DropoutMask mask;
+    explicit GatedProduct(std::vector<Node*>& inputs, Activation activation, const DropoutMask& mask);
+    ~GatedProduct() override;
+    bool canOverwriteGradient(size_t) override { return true; }
+    Shape checkShape(std::vector<Shape>& inputShapes) override;
+    void forward(const std::vector<const Tensor*>& inputs, Tensor* output) override;
+    using Function::forward;
+    void backward() override;  // both gradients from one pass over the kept products
+
+private:
+    Device* device = nullptr;
+    void* pre = nullptr;  // both products, kept for the backward pass when an input has a gradient
+};
+
+// inputs: x, or x and the residual it is added to
+class DEEP8_API Dropout : public Function {
+public:
+    DropoutMask mask;
+    explicit Dropout(std::vector<Node*>& inputs, const DropoutMask& mask);
+    bool canOverwriteGradient(size_t) override { return true; }
+    Shape checkShape(std::vector<Shape>& inputShapes) override;
+    void forward(const std::vector<const Tensor*>& inputs, Tensor* output) override;
+    void backward(const std::vector<const Tensor*>& inputs, const Tensor* output, const Tensor* outputGradient, size_t index,
+                  Tensor* iGradient) override;
+    using Function::forward;
+    using Function::backward;
+};
+
+class DEEP8_API RMSNorm : public Function {
+public:
+    float epsilon;
+    explicit RMSNorm(std::vector<Node*>& inputs, float epsilon);
+    ~RMSNorm() override;
+    bool canOverwriteGradient(size_t) override { return true; }
+    Shape checkShape(std::vector<Shape>& inputShapes) override;
+    void forward(const std::vector<const Tensor*>& inputs, Tensor* output) override;
+    using Function::forward;
+    void backward() override;
+
+private:
+    Device* device = nullptr;
+    float* rstd = nullptr;
 };
 
 // ------------------------------------------------------------------------------------------------ executors
@@ -610,6 +687,11 @@ DEEP8_API Variable& conv2d(Variable& x, Variable& filter, bool covered = true, i
 DEEP8_API Variable& deConv2d(Variable& x, Variable& filter, bool covered = false, int strideY = 1, int strideX = 1);
 DEEP8_API Variable& relu(Variable& x);
 DEEP8_API Variable& linear(Variable& x, float a = 1, float b = 0);
+// additions: dropout(activation(x * w[0]) * (x * w[1])), (residual +) dropout(x), x / rms(x) * weight
+DEEP8_API Variable& gatedProduct(Variable& x, Variable& w, Activation activation = Activation::SiLu, const DropoutMask& mask = DropoutMask());
+DEEP8_API Variable& dropout(Variable& x, const DropoutMask& mask);
+DEEP8_API Variable& dropout(Variable& x, const DropoutMask& mask, Variable& residual);
+DEEP8_API Variable& rmsNorm(Variable& x, Variable& weight, float epsilon = 1e-6f);
 DEEP8_API Variable& operator+(Variable& x, Variable& y);
 DEEP8_API Variable& add(Variable& x, Variable& y);
 

@@ -9,6 +9,8 @@ dropped).  The activations are good to 2^-18 of (1 + |a|) times their size: the 
 rounded argument z by 2 z^2 * 2^-24 < 2^-18 for |z| < 5.
 """
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -799,3 +801,12 @@ def test_gated_beyond_32_bit_offsets(ctx):
         # sums differ by 2 * 64 * 2^-23 * 64 * 3.9 < 2^-8.0 at the very most, times the other factor (below 16)
         assert ((got[keep] - want).abs() <= want.abs() * 2.0 ** -9.9 + 2.0 ** -8 * 16).all()
     assert ctx.status() == 0
+
+
+@pytest.mark.gpu
+def test_cpp_nodes():
+    """The C++ nodes (tests/cpp/test_feedforward_host.cu): the block as a graph, forward and backward walk."""
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "test_feedforward_host")
+    assert os.path.exists(exe), "tests/cpp/bin/test_feedforward_host is missing: run __graft_entry__.build()"
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
