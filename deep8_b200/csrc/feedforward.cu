@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(256) pad_kernel(PadJobs jobs, int count) {
         const size_t total = static_cast<size_t>(jobs.job[q].rows) * packs;
         const uintptr_t lowest = reinterpret_cast<uintptr_t>(src), highest = lowest + static_cast<size_t>(jobs.job[q].rows) * cols * sizeof(T);
         for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
-            const size_t r = i / packs;
+            const size_t r = total <= 0xffffffffu ? static_cast<unsigned>(i) / static_cast<unsigned>(packs) : i / packs;
             const int c = static_cast<int>(i - r * packs) * W;
             const T* from = src + r * cols + c;
             const uintptr_t piece = reinterpret_cast<uintptr_t>(from) & ~static_cast<uintptr_t>(15);
@@ -328,12 +328,20 @@ __global__ void __launch_bounds__(256) gated_grad_pre_kernel(const T* pre, const
                 store_pack(dpre + i0, g);
                 store_pack(dpre + n + i0, u);
             } else {
+                // rows of dpre may be padded: where this step's first element goes
+                const size_t r = n <= 0xffffffffu ? static_cast<unsigned>(i0) / width : i0 / width;
+                unsigned col = static_cast<unsigned>(i0 - r * width);
+                size_t at = r * pitch + col;
 #pragma unroll
                 for (int k = 0; k < E; ++k)
                     if (i0 + k < n) {
-                        const size_t r = (i0 + k) / width, at = r * pitch + (i0 + k - r * width);  // rows of dpre may be padded
                         dpre[at] = g.v[k];
                         dpre[second + at] = u.v[k];
+                        ++at;
+                        if (++col == width) {  // on to the next row, `pitch` further than the last one began
+                            col = 0;
+                            at += pitch - width;
+                        }
                     }
             }
         }
@@ -700,8 +708,10 @@ int resident_ctas(Kernel* kernel, int threads, size_t dyn = 0) {
 // ran a second, emptier round (dropout 49 us for 37).
 template <class Kernel>
 unsigned grid_for(const d8k_ctx* ctx, Kernel* kernel, size_t steps) {
-    const size_t blocks = (steps + 255) / 256, cap = static_cast<size_t>(ctx->num_sms) * resident_ctas(kernel, 256);
-    return static_cast<unsigned>(blocks > cap ? cap : blocks < 1 ? 1 : blocks);
+    const size_t blocks = (steps + 255) / 256;
+    if (blocks <= static_cast<size_t>(ctx->num_sms)) return static_cast<unsigned>(blocks < 1 ? 1 : blocks);
+    const size_t cap = static_cast<size_t>(ctx->num_sms) * resident_ctas(kernel, 256);
+    return static_cast<unsigned>(blocks > cap ? cap : blocks);
 }
 
 // The launch's form of a dropout argument; *on stays 0 when there is nothing to drop (none given, or p == 0).
@@ -725,7 +735,7 @@ int make_drop(const d8k_dropout* drop, DropSpec* spec, int* on) {
 int check_gated(int activation, int xb, int xr, int xc, int yc) {
     if (activation < 0 || activation >= kActCount) return fail(D8K_ERR_ARGUMENT, "gated: no such activation");
     if (xb < 0 || xr < 0 || xc < 1 || yc < 1) return fail(D8K_ERR_ARGUMENT, "the shape is error");
-    if (1LL * xb * xr >= (1LL << 31)) return fail(D8K_ERR_ARGUMENT, "the shape is too large");
+    if (1LL * xb * xr > (1LL << 30) || xc > (1 << 30) || yc > (1 << 30)) return fail(D8K_ERR_ARGUMENT, "the shape is too large");
     return 0;
 }
 
@@ -940,7 +950,7 @@ int rms_norm_forward(d8k_ctx* ctx, const T* x, const T* weight, float eps, T* y,
                                                                                                             : rms_norm_forward_kernel<T, W, 4>)
                           : (p.packs_per_thread == 1 ? rms_norm_forward_kernel<T, 1, 1> : p.packs_per_thread == 4 ? rms_norm_forward_kernel<T, 1, 4>
                                                                                                             : rms_norm_forward_kernel<T, 1, 16>);
-        const size_t cap = static_cast<size_t>(ctx->num_sms) * resident_ctas(kernel, p.threads);
+        const size_t sms = ctx->num_sms, cap = groups <= sms ? sms : sms * resident_ctas(kernel, p.threads);
         kernel<<<static_cast<unsigned>(groups < cap ? groups : cap), p.threads, 0, ctx->stream>>>(x, weight, y, rstd, rows, cols, eps, p.tpr);
     }
     D8K_CUDA(cudaGetLastError());

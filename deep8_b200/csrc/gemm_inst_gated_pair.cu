@@ -41,8 +41,8 @@ __global__ void __launch_bounds__(256) split_sum_kernel(const SplitSum q) {
     const size_t stride = static_cast<size_t>(q.batch) * q.tiles_m * q.tiles_n * 65536;
     const unsigned long long offset = GATED && q.gated.dropping ? drop_offset(q.gated.drop) : 0;
     for (size_t i = blockIdx.x * 256ull + threadIdx.x; i < total; i += gridDim.x * 256ull) {
-        const size_t line = i / quads;
-        const int c = static_cast<int>(i - line * quads) * 4, b = static_cast<int>(line / q.M), r = static_cast<int>(line - static_cast<size_t>(b) * q.M);
+        const size_t line = total <= 0xffffffffu ? static_cast<unsigned>(i) / quads : i / quads;
+        const int c = static_cast<int>(i - line * quads) * 4, b = q.batch == 1 ? 0 : static_cast<int>(line / q.M), r = static_cast<int>(line - static_cast<size_t>(b) * q.M);
         const size_t tile = (static_cast<size_t>(b) * q.tiles_m + r / 256) * q.tiles_n + c / TILE_N;
         const float* src = q.ws + (tile * 256 + r % 256) * 256 + c % TILE_N;
         const float4 first = sum_slices(src, q.splits, stride);
