@@ -150,6 +150,18 @@ __device__ __forceinline__ __half ld_shared_half(uint32_t addr) {
     return __ushort_as_half(v);
 }
 
+// A staging slot's 32 rows to memory, one row per store and a column per lane; `to` is this lane's column of the first row.  Rows and columns from
+// `rows` and `cols` on are left out.
+__device__ __forceinline__ void store_slot_rows(__half* to, long long ldc, uint32_t slot, int lane, int rows, int cols) {
+    if (lane >= cols) return;
+    if (rows >= 32) {
+#pragma unroll
+        for (int rr = 0; rr < 32; ++rr) to[rr * ldc] = ld_shared_half(slot + slot_off(rr, lane >> 3) + 2 * (lane & 7));
+    } else {
+        for (int rr = 0; rr < rows; ++rr) to[rr * ldc] = ld_shared_half(slot + slot_off(rr, lane >> 3) + 2 * (lane & 7));
+    }
+}
+
 struct PairWork {
     int batch, m0, n0;
 };
@@ -465,10 +477,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 #pragma unroll
                         for (int k = 0; k < 4; ++k) st_shared_v4(slot + slot_off(lane, k), V::pack(v + 8 * k));
                         __syncwarp();
-#pragma unroll 4
-                        for (int rr = 0; rr < 32; ++rr)
-                            if (warp_row0 + rr < p.M && col0 + lane < p.N)
-                                out[static_cast<long long>(rr) * p.ldc + col0 + lane] = ld_shared_half(slot + slot_off(rr, lane >> 3) + 2 * (lane & 7));
+                        store_slot_rows(out + col0 + lane, p.ldc, slot, lane, p.M - warp_row0, p.N - col0);
                     }
                 }
             } else if constexpr (Cfg::GATED) {
@@ -500,10 +509,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         // rows that start anywhere, or end inside these columns: one row per store, a column per lane
                         auto rows_out = [&](OutT* dst, uint32_t slot) {
                             __syncwarp();
-#pragma unroll 4
-                            for (int rr = 0; rr < 32; ++rr)
-                                if (warp_row0 + rr < p.M && col0 + lane < p.N)
-                                    dst[static_cast<long long>(warp_row0 + rr) * p.ldc + col0 + lane] = ld_shared_half(s0 + slot + slot_off(rr, lane >> 3) + 2 * (lane & 7));
+                            store_slot_rows(dst + static_cast<long long>(warp_row0) * p.ldc + col0 + lane, p.ldc, s0 + slot, lane, p.M - warp_row0, p.N - col0);
                             __syncwarp();
                         };
                         if (t.pre) {
