@@ -505,6 +505,8 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     if (col0 >= p.N) continue;
                     const uint32_t s0 = staging, s1 = staging + Cfg::SLOT_BYTES;
                     using V = EpiVec<OutT>;
+                    const uint32_t stays =
+                        t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0) : 0xffffffffu;
                     if (!segments || col0 + 32 > p.N) {
                         // rows that start anywhere, or end inside these columns: one row per store, a column per lane
                         auto rows_out = [&](OutT* dst, uint32_t slot) {
@@ -521,7 +523,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                             rows_out(reinterpret_cast<OutT*>(t.pre), 0);
                             rows_out(reinterpret_cast<OutT*>(t.pre) + t.pre_stride, Cfg::SLOT_BYTES);
                         }
-                        gated_values<OutT>(t, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0, gate, up);
+                        gated_values<OutT>(t, stays, gate, up);
 #pragma unroll
                         for (int v = 0; v < 4; ++v) st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
                         rows_out(reinterpret_cast<OutT*>(p.C), 0);
@@ -546,7 +548,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         }
                         __syncwarp();
                     }
-                    gated_values<OutT>(t, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0, gate, up);
+                    gated_values<OutT>(t, stays, gate, up);
 #pragma unroll
                     for (int v = 0; v < 4; ++v) st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
                     __syncwarp();

@@ -809,9 +809,9 @@ __device__ __forceinline__ uint32_t drop_mask32(const DropSpec& d, unsigned long
     return bits;
 }
 
-// gate[i] = dropout(act(gate[i]) * up[i]) for 32 consecutive elements, the first of them element `first` of h
+// gate[i] = dropout(act(gate[i]) * up[i]) for 32 elements; bit i of `stays`: the dropout's decision
 template <typename OutT>
-__device__ __forceinline__ void gated_values(const GatedTail& t, unsigned long long first, float* gate, const float* up) {
+__device__ __forceinline__ void gated_values(const GatedTail& t, uint32_t stays, float* gate, const float* up) {
     with_activation(t.act, [&](auto act) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
@@ -821,40 +821,83 @@ __device__ __forceinline__ void gated_values(const GatedTail& t, unsigned long l
         }
     });
     if (t.dropping) {
-        const uint32_t stays = drop_mask32(t.drop, first);
 #pragma unroll
         for (int i = 0; i < 32; ++i) gate[i] = (stays >> i & 1u) ? gate[i] * t.drop.scale : 0.0f;
     }
 }
 
-// Tail of a gated product for one row and 32 columns [col0, col0 + 32), clipped to N: both projections (when kept) and h, each rounded
-// once.  Overwrites gate.
+// v[c] of lane r <-> v[r] of lane c (whole warp): afterwards a lane holds one column of 32 rows, and a store of v[r] by all lanes writes a whole
+// segment of row r.  Rows that start anywhere would otherwise leave as 32 stores of single elements in 32 rows each (333 x 250 x 1001
+// fp16: 8 us per stored tensor).
+__device__ __forceinline__ void transpose32(float* v, int lane) {
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) {
+        const bool high = lane & s;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            if (i & s) continue;
+            const float got = __shfl_xor_sync(0xffffffffu, high ? v[i] : v[i + s], s);
+            if (high) v[i] = got;
+            else v[i + s] = got;
+        }
+    }
+}
+// v[r] to row r, this lane's column at `to`; rows and columns from `rows` and `cols` on are left out
 template <typename OutT>
-__device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, int col0, float* gate, const float* up) {
+__device__ __forceinline__ void store_transposed(OutT* to, long long ld, const float* v, int lane, int rows, int cols) {
+    if (lane >= cols) return;
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+        if (r < rows) to[r * ld] = epi_from_float<OutT>(v[r]);
+}
+
+// Tail of a gated product for a warp's 32 rows (this lane's is `row`, which may be past the last) and 32 columns [col0, col0 + 32), clipped to N: both
+// projections (when kept) and h, each rounded once.  Called by whole warps; overwrites gate and up.
+template <typename OutT>
+__device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, int col0, float* gate, float* up) {
     using V = EpiVec<OutT>;
     constexpr int VEC = V::N;
     const GatedTail& t = p.gated;
     const long long off = static_cast<long long>(row) * p.ldc + col0;
+    uint32_t stays = t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(off)) : 0xffffffffu;
     OutT* h = reinterpret_cast<OutT*>(p.C) + off;
-    OutT* pg = t.pre ? reinterpret_cast<OutT*>(t.pre) + off : nullptr;
-    OutT* pu = t.pre ? pg + t.pre_stride : nullptr;
-    const bool vec_ok = col0 + 32 <= p.N && ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(pg) | reinterpret_cast<uintptr_t>(pu)) & 15) == 0;
-    auto store = [&](OutT* dst, const float* v) {
-        if (vec_ok) {
+    OutT* pre = reinterpret_cast<OutT*>(t.pre) + off;
+    const bool vec_ok = col0 + 32 <= p.N && ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(t.pre)) & 15) == 0 && p.ldc % VEC == 0 &&
+                        t.pre_stride % VEC == 0;
+    if (vec_ok) {
+        auto store = [&](OutT* dst, const float* v) {
+            if (row < p.M) {
 #pragma unroll
-            for (int k = 0; k < 32 / VEC; ++k) reinterpret_cast<uint4*>(dst)[k] = V::pack(v + k * VEC);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)  // fully unrolled: a dynamic index would push the accumulators to local memory
-                if (col0 + i < p.N) dst[i] = epi_from_float<OutT>(v[i]);
+                for (int k = 0; k < 32 / VEC; ++k) reinterpret_cast<uint4*>(dst)[k] = V::pack(v + k * VEC);
+            }
+        };
+        if (t.pre) {
+            store(pre, gate);
+            store(pre + t.pre_stride, up);
         }
-    };
-    if (pg) {
-        store(pg, gate);
-        store(pu, up);
+        gated_values<OutT>(t, stays, gate, up);
+        store(h, gate);
+    } else {
+        const int lane = threadIdx.x & 31, rows = p.M - (row - lane), cols = p.N - col0;
+        const long long first = static_cast<long long>(row - lane) * p.ldc + col0 + lane;
+        transpose32(gate, lane);
+        transpose32(up, lane);
+        if (t.dropping) {  // the decisions change places, too
+            uint32_t column = 0;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const uint32_t bits = __ballot_sync(0xffffffffu, stays >> i & 1u);
+                if (lane == i) column = bits;
+            }
+            stays = column;
+        }
+        if (t.pre) {
+            store_transposed(reinterpret_cast<OutT*>(t.pre) + first, p.ldc, gate, lane, rows, cols);
+            store_transposed(reinterpret_cast<OutT*>(t.pre) + t.pre_stride + first, p.ldc, up, lane, rows, cols);
+        }
+        gated_values<OutT>(t, stays, gate, up);
+        store_transposed(reinterpret_cast<OutT*>(p.C) + first, p.ldc, gate, lane, rows, cols);
     }
-    gated_values<OutT>(t, static_cast<unsigned long long>(off), gate, up);
-    store(h, gate);
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
@@ -1265,7 +1308,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                             ptx::tmem_ld_32x32(taddr + c * 32, r);
                             ptx::tmem_ld_32x32(taddr + BN / 2 + c * 32, s);
                             ptx::tmem_ld_wait();
-                            if (row_ok && it.n0 / 2 + c * 32 < p.N) {
+                            if (it.n0 / 2 + c * 32 < p.N) {
                                 float gate[32], up[32];
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
@@ -1338,7 +1381,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                 }
                 if (!ok) break;
                 if constexpr (Cfg::GATED) {
-                    if (p.splits == 1 && row_ok) {
+                    if (p.splits == 1) {
 #pragma unroll
                         for (int c = 0; c < BN / 64; ++c)
                             if (it.n0 / 2 + c * 32 < p.N) store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, &accv[c * 32], &accv[BN / 2 + c * 32]);
@@ -1385,7 +1428,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (s_last) {
                     __threadfence();
-                    if (row_ok) {
+                    if (Cfg::GATED || row_ok) {
                         const float* first = p.ws + (static_cast<size_t>(it.tile) * p.splits * kBM + row_in_tile) * BN;
                         if constexpr (Cfg::GATED) {
 #pragma unroll 1

@@ -655,9 +655,10 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
 
 // How the gated block's fp16 products run: 0 on the one-CTA kernel, 1 on the paired kernel, more on the paired kernel in that many slices.
 // A model in us, from measured times.  Paired: a stage (128 k) of a 256 x 256 tile 0.76, but a tile not less than `store`, its epilogue; one-CTA: a
-// k-block of 64 on a 128 x 128 tile 0.5, whatever it multiplies, a tile not less than 2.5.  6 for a launch with its fill and drain; for slices 3 for the
+// k-block of 64 on a 128 x 128 tile 0.5, whatever it multiplies, a tile not less than 2.5, and 8 more where its rows leave element by element
+// (`ragged`: run_gemm's kernels; the paired ones and the gated ones store such rows in segments).  6 for a launch with its fill and drain; for slices 3 for the
 // sum's launch and its reads at 3 TB/s.  `tiles` counts 256 x 256 tiles, `singles` the one-CTA kernel's, `its` stages.
-static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int its, double store) {
+static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int its, double store, bool ragged) {
     const int pairs = ctx->num_sms / 2;
     auto rounds = [](long long work, int at_once) { return static_cast<double>((work + at_once - 1) / at_once); };
     auto longer = [](double a, double b) { return a > b ? a : b; };
@@ -671,7 +672,7 @@ static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int i
             extra = 4;
         }
     }
-    double best = rounds(singles, ctx->num_sms) * longer(kb * 0.5, 2.5) + 6 + extra;
+    double best = rounds(singles, ctx->num_sms) * (longer(kb * 0.5, 2.5) + (ragged ? 8 : 0)) + 6 + extra;
     int choice = 0;
     const double unsplit = rounds(tiles, pairs) * longer(its * 0.76, store) + 6;
     if (unsplit < best) {
@@ -703,7 +704,8 @@ int run_gated_grad(Ctx* ctx, const GemmProblem& g) {
         return run_gemm(ctx, g);
     const long long singles = static_cast<long long>(g.batch) * ((g.M + 127LL) / 128) * ((g.N + 127LL) / 128);
     const int num_kb = (g.K + 63) / 64, its = g.kbatch * ((num_kb + 1) / 2);
-    const int slices = pair_slices(ctx, tiles, singles, its, 3.0);
+    const bool ragged = ((g.ldc | g.c_batch_stride) & 7) != 0 || (reinterpret_cast<uintptr_t>(g.C) & 15) != 0;
+    const int slices = pair_slices(ctx, tiles, singles, its, 3.0, ragged);
     if (slices == 0) return run_gemm(ctx, g);
     GemmParams p;
     std::memset(&p, 0, sizeof(p));
@@ -822,7 +824,7 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     // fp16: the paired kernel, whole (1) or in slices, where the model finds it faster
     int slices = 0;
     if (can_tma && !f32 && g.M > 128 && env_int("D8K_PAIR", 1) != 0 && ptiles < (1LL << 30))
-        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, 5.0);
+        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, 5.0, false);
     // The paired kernel reads rows of whole 128-byte pieces: x is copied with padded rows for it, w from 4096 rows on, where the product dwarfs the copy
     bool pad_a = !tma_ok(a, esize) || (slices && g.K % bk != 0);
     const bool pad_b = !tma_ok(b, esize) || (slices && g.N % bk != 0 && g.M >= 4096);
