@@ -827,9 +827,9 @@ int gated_operands(d8k_ctx* ctx, int dtype, GatedOperands* o, const void* x, con
     bool wanted[3] = {};
     for (int k = 0; k < 3; ++k) {
         // Rows of whole 128-byte pieces as well where that lets a faster kernel read them: x (a small copy) for the paired kernel or, in fp32, any TMA
-        // kernel; dpre for the same when it costs no copy, in fp32 always; w from 4096 rows on, where the product dwarfs the copy.
+        // kernel; dpre for the same when it costs no copy, in fp32 always; w where the paired kernel saves more than the copy costs.
         const bool whole = parts[k].cols % piece == 0;
-        const bool useful = !whole && (k == 0 || (k == 1 ? dtype == D8K_F16 && rows >= 4096 : dpre_to_come || dtype == D8K_F32));
+        const bool useful = !whole && (k == 0 || (k == 1 ? dtype == D8K_F16 && gated_grad_x_wants_padded_w(ctx, rows, xc, yc) : dpre_to_come || dtype == D8K_F32));
         wanted[k] = parts[k].o->ptr && (useful || !rows_aligned(parts[k].o->ptr, parts[k].cols, dtype));
         at[k] = bytes;
         if (wanted[k]) bytes += (static_cast<size_t>(parts[k].rows) * ((parts[k].cols + piece - 1) / piece * piece) * esize(dtype) + 255) & ~static_cast<size_t>(255);

@@ -88,6 +88,8 @@ struct PadJob {
 void* pad_memory(Ctx* ctx, size_t bytes);
 // up to two copies in one launch (feedforward.cu)
 cudaError_t launch_pad(Ctx* ctx, int dtype, const PadJob* jobs, int count);
+// whether the paired kernel saves the fp16 gradient of x more than a copy of w with padded rows costs
+bool gated_grad_x_wants_padded_w(const Ctx* ctx, int rows, int xc, int yc);
 // whether TMA can describe a stored matrix stack of rows of `ld` elements at ptr
 bool rows_aligned(const void* ptr, long long ld, int dtype);
 

@@ -658,7 +658,8 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
 // k-block of 64 on a 128 x 128 tile 0.5, whatever it multiplies, a tile not less than 2.5, and 8 more where its rows leave element by element
 // (`ragged`: run_gemm's kernels; the paired ones and the gated ones store such rows in segments).  6 for a launch with its fill and drain; for slices 3 for the
 // sum's launch and its reads at 3 TB/s.  `tiles` counts 256 x 256 tiles, `singles` the one-CTA kernel's, `its` stages.
-static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int its, double store, bool ragged) {
+// *gain: what the choice saves over the one-CTA kernel.
+static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int its, double store, bool ragged, double* gain = nullptr) {
     const int pairs = ctx->num_sms / 2;
     auto rounds = [](long long work, int at_once) { return static_cast<double>((work + at_once - 1) / at_once); };
     auto longer = [](double a, double b) { return a > b ? a : b; };
@@ -672,7 +673,8 @@ static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int i
             extra = 4;
         }
     }
-    double best = rounds(singles, ctx->num_sms) * (longer(kb * 0.5, 2.5) + (ragged ? 8 : 0)) + 6 + extra;
+    const double single = rounds(singles, ctx->num_sms) * (longer(kb * 0.5, 2.5) + (ragged ? 8 : 0)) + 6 + extra;
+    double best = single;
     int choice = 0;
     const double unsplit = rounds(tiles, pairs) * longer(its * 0.76, store) + 6;
     if (unsplit < best) {
@@ -690,7 +692,17 @@ static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int i
             choice = s;
         }
     }
+    if (gain) *gain = single - best;
     return choice;
+}
+
+// A padded copy of `bytes` in us: its launch, and reading and writing at 3 TB/s
+static double pad_cost(double bytes) { return 3 + 2 * bytes / 3e6; }
+
+bool gated_grad_x_wants_padded_w(const Ctx* ctx, int rows, int xc, int yc) {
+    const long long tiles = (rows + 255LL) / 256 * ((xc + 255LL) / 256), singles = (rows + 127LL) / 128 * ((xc + 127LL) / 128);
+    double gain = 0;
+    return tiles < (1LL << 30) && pair_slices(ctx, tiles, singles, 2 * ((yc + 127) / 128), 3.0, xc % 8 != 0, &gain) != 0 && gain > pad_cost(4.0 * xc * yc);
 }
 
 int run_gated_grad(Ctx* ctx, const GemmProblem& g) {
@@ -823,11 +835,12 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     const int its = (g.K + 127) / 128;
     // fp16: the paired kernel, whole (1) or in slices, where the model finds it faster
     int slices = 0;
+    double gain = 0;
     if (can_tma && !f32 && g.M > 128 && env_int("D8K_PAIR", 1) != 0 && ptiles < (1LL << 30))
-        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, 5.0, false);
-    // The paired kernel reads rows of whole 128-byte pieces: x is copied with padded rows for it, w from 4096 rows on, where the product dwarfs the copy
+        slices = pair_slices(ctx, ptiles, mtiles * ((g.N + 63LL) / 64), its, 5.0, false, &gain);
+    // The paired kernel reads rows of whole 128-byte pieces: x and w are copied with padded rows where it saves more than that costs
     bool pad_a = !tma_ok(a, esize) || (slices && g.K % bk != 0);
-    const bool pad_b = !tma_ok(b, esize) || (slices && g.N % bk != 0 && g.M >= 4096);
+    const bool pad_b = !tma_ok(b, esize) || (slices && g.N % bk != 0 && gain > pad_cost(4.0 * g.K * g.N));
     if (!pad_b && g.N % bk != 0) pad_a = !tma_ok(a, esize);  // x alone would not do
     if (can_tma && (pad_a || pad_b)) {
         // Rows that do not start on 16-byte boundaries: copies with padded rows, read by TMA.  The loader warps fetch such rows element by
