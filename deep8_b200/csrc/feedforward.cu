@@ -63,9 +63,10 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {  // read once: not
 // The gated product for R rows of x at most (a token, or a few, while a model answers): bound by reading both weight matrices once, so
 // no tensor cores.  A CTA takes a strip of 16 packs of columns (of 16 bytes) and a slice of the contraction; its 16 groups of 16 threads
 // take every 16th k, each thread a pack of both projections, R products each in fp32.  The groups' sums meet in shared memory, the slices'
-// in scratch memory: the CTA that finishes a strip last adds them in slice order and forms h.
+// in scratch memory: the CTA that finishes a strip last adds them in slice order and forms h.  fp32, 4096 -> 2 x 16384: 82 us for one row
+// (6.5 TB/s), 88 for two to four, 146 for eight, whose multiply-adds no longer fit behind the loads; the tensor cores take 228 us.
 template <typename T, int R>
-__global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T* __restrict__ x, const T* __restrict__ w, T* __restrict__ h, int rows_all, int cols,
+__global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T* __restrict__ x, const T* __restrict__ w, T* __restrict__ h, int rows, int cols,
                                                          int width, int k_per_slice, float* __restrict__ partial, unsigned* arrivals, GatedTail tail) {
     constexpr int V = 16 / sizeof(T), STRIP = 16 * V;
     constexpr int CHUNK = R > 4 ? 256 : 512;  // k staged at a time
@@ -73,10 +74,6 @@ __global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T*
     __shared__ float sums[8][2 * R * V][16];
     const int lane = threadIdx.x & 15, kl = threadIdx.x >> 4;
     const int c = blockIdx.x * STRIP + lane * V;
-    const int row0 = blockIdx.z * R, rows = min(rows_all - row0, R);  // this group of rows
-    x += static_cast<size_t>(row0) * cols;
-    arrivals += static_cast<size_t>(blockIdx.z) * gridDim.x;
-    partial += static_cast<size_t>(blockIdx.z) * gridDim.x * gridDim.y * (2 * R * STRIP);
     const int k_begin = blockIdx.y * k_per_slice, k_end = min(cols, k_begin + k_per_slice);
     const size_t second = static_cast<size_t>(cols) * width;
     float g[R][V] = {}, u[R][V] = {};
@@ -167,7 +164,7 @@ __global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T*
             gate = summed(i, 0);
             up = summed(i, 1);
         }
-        const size_t at = static_cast<size_t>(row0 + r) * width + col;
+        const size_t at = static_cast<size_t>(r) * width + col;
         if (tail.pre) {
             static_cast<T*>(tail.pre)[at] = narrow<T>(gate);
             static_cast<T*>(tail.pre)[tail.pre_stride + at] = narrow<T>(up);
@@ -739,26 +736,25 @@ int check_gated(int activation, int xb, int xr, int xc, int yc) {
     return 0;
 }
 
-// The fp32 product for up to 16 rows in groups of one, two, four or eight, true when it is this kernel's: whole 16-byte packs of columns at
-// 16-byte boundaries, and strips few enough for the arrival words.  (fp16 has gemm_gated_few.cu, which reads as fast for any of these row
-// counts.)  As many slices as are in work at once, of at least 64 k.
+// The fp32 product for up to eight rows (nine would be two passes, 292 us where the tensor cores take 228), true when it is this kernel's: whole
+// 16-byte packs of columns at 16-byte boundaries, and strips few enough for the arrival words.  (fp16 has gemm_gated_few.cu, which
+// reads as fast for any of these row counts.)  As many slices as are in work at once, of at least 64 k.
 bool gated_rows(d8k_ctx* ctx, const float* x, const float* w, float* h, int rows, int cols, int width, const GatedTail& tail) {
     constexpr int V = 4;
-    const int strips = (width + 16 * V - 1) / (16 * V), groups = (rows + 7) / 8;
-    if (rows > 8 || width % V != 0 || !aligned16({w}) || strips * groups > kMaxCounters) return false;
+    const int strips = (width + 16 * V - 1) / (16 * V);
+    if (rows > 8 || width % V != 0 || !aligned16({w}) || strips > kMaxCounters) return false;
     const int r = rows <= 2 ? rows : rows <= 4 ? 4 : 8;
     auto kernel = r == 1 ? gated_rows_kernel<float, 1> : r == 2 ? gated_rows_kernel<float, 2> : r == 4 ? gated_rows_kernel<float, 4> : gated_rows_kernel<float, 8>;
-    long long slices = static_cast<long long>(ctx->num_sms) * resident_ctas(kernel, 256) / (strips * groups);
+    long long slices = static_cast<long long>(ctx->num_sms) * resident_ctas(kernel, 256) / strips;
     if (slices > cols / 64) slices = cols / 64;
-    const long long most = static_cast<long long>(ctx->scratch_bytes / (static_cast<size_t>(strips) * groups * 2 * r * 16 * V * sizeof(float)));
+    const long long most = static_cast<long long>(ctx->scratch_bytes / (static_cast<size_t>(strips) * 2 * r * 16 * V * sizeof(float)));
     if (slices > most) slices = most;
     if (slices > 255) slices = 255;
     if (slices < 1) slices = 1;
     int per = static_cast<int>((cols + slices - 1) / slices);
     per = (per + 15) / 16 * 16;
     slices = (cols + per - 1) / per;
-    kernel<<<dim3(strips, static_cast<unsigned>(slices), groups), 256, 0, ctx->stream>>>(x, w, h, rows, cols, width, per, ctx->scratch,
-                                                                               ctx->arrivals, tail);
+    kernel<<<dim3(strips, static_cast<unsigned>(slices)), 256, 0, ctx->stream>>>(x, w, h, rows, cols, width, per, ctx->scratch, ctx->arrivals, tail);
     return true;
 }
 
@@ -1020,6 +1016,13 @@ void* pad_memory(Ctx* ctx, size_t bytes) {
         return nullptr;
     }
     if (capturing != cudaStreamCaptureStatusNone) return nullptr;
+    // another stream may be under capture, by this thread or another: an allocation would end it in the global mode
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    struct Restore {
+        cudaStreamCaptureMode* mode;
+        ~Restore() { cudaThreadExchangeStreamCaptureMode(mode); }
+    } restore{&mode};
     size_t want = ctx->pad_bytes * 2 > bytes ? ctx->pad_bytes * 2 : bytes;  // the sum of all stays below twice the last
     if (want < (static_cast<size_t>(16) << 20)) want = static_cast<size_t>(16) << 20;
     ctx->pads.reserve(ctx->pads.size() + 1);

@@ -21,6 +21,8 @@
 // whatever their size (16 KB or 32 KB), so a stage holds SUB = 2 k-blocks of 64 and each operand arrives as ONE 32 KB box
 // of a 4-D tensor map {64 elements, rows, k-blocks (or 64-element chunks), batch}; with 16 KB boxes (one k-block per
 // stage) the tensor pipe waited on operand delivery a third of the time.
+// Three further forms (Gemm2Cfg): GATED, the gated projection pair, one CTA of the pair per projection; SPLIT, slices of a long contraction
+// over few tiles, summed by a second launch; STORE8, eight epilogue warps for short contractions.
 // No load uses multicast.  Every wait is bounded as in the single-CTA kernel; the two cluster barriers (after set-up,
 // before tensor memory is freed) are reached by every thread on every path.
 #pragma once

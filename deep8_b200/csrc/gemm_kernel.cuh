@@ -28,6 +28,10 @@
 // split; TWIN - one CTA per SM with two TMA-issuing threads (A's boxes, B's boxes) and two MMA-issuing threads that take
 // k-blocks in turn under a token, for every other TMA launch.  Both keep the order in which the sums are formed.
 //
+// GATED: B is a pair of matrices and a tile's columns are half of each, so that one accumulator row holds both projections of the same
+// outputs; the epilogue forms act(gate) * up, the dropout, and stores the projections too when the backward pass is to come.
+// PRECISE (fp32): chains of four k-blocks instead of sixteen per fp32 sum, the small terms in columns of their own.
+//
 // Every mbarrier wait is bounded: on expiry the CTA records a status code, all roles leave their loops, and the
 // kernel returns through the normal teardown (TMEM freed).
 #pragma once
@@ -1292,7 +1296,9 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
             const int row = it.m0 + row_in_tile;
             const bool row_ok = out_row_exists(p, row);
             const long long crow = static_cast<long long>(it.batch) * p.c_batch_stride + out_row_offset(p, row) + scatter_offset(p, row);
-            float* part = p.ws + (static_cast<size_t>(w) * kBM + row_in_tile) * BN;
+            // A partial tile of a split contraction, read by the thread of the same row that it was written by: four columns of all rows
+            // together, so that a warp's accesses are whole lines
+            float* part = p.ws + static_cast<size_t>(w) * kBM * BN + row_in_tile * 4;
             if constexpr (Cfg::CHUNK_KB == 0) {
                 ok = wait_bar_timed(tfull_bar(acc), acc_phase, &s_abort, p.status, (kRoleEpilogue << 8) | 3, timed, &w_tfull,
                                     static_cast<unsigned>(p.epi_backoff_ns));
@@ -1336,7 +1342,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                     } else {
 #pragma unroll
                         for (int v = 0; v < 8; ++v)
-                            __stcg(reinterpret_cast<uint4*>(part + c * 32) + v, make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]));
+                            __stcg(reinterpret_cast<uint4*>(part + (c * 8 + v) * (kBM * 4)), make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]));
                     }
                 }
                 ptx::tc_fence_before_sync();
@@ -1395,7 +1401,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                     } else {
 #pragma unroll
                         for (int v = 0; v < 8; ++v)
-                            __stcg(reinterpret_cast<float4*>(part + c * 32) + v,
+                            __stcg(reinterpret_cast<float4*>(part + (c * 8 + v) * (kBM * 4)),
                                    make_float4(accv[c * 32 + 4 * v], accv[c * 32 + 4 * v + 1], accv[c * 32 + 4 * v + 2], accv[c * 32 + 4 * v + 3]));
                     }
                 }
@@ -1429,7 +1435,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                 if (s_last) {
                     __threadfence();
                     if (Cfg::GATED || row_ok) {
-                        const float* first = p.ws + (static_cast<size_t>(it.tile) * p.splits * kBM + row_in_tile) * BN;
+                        const float* first = p.ws + static_cast<size_t>(it.tile) * p.splits * kBM * BN + row_in_tile * 4;
                         if constexpr (Cfg::GATED) {
 #pragma unroll 1
                             for (int c = 0; c < BN / 64; ++c) {
@@ -1438,10 +1444,10 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) gate[i] = up[i] = 0.f;
                                 for (int s = 0; s < p.splits; ++s) {
-                                    const float4* src = reinterpret_cast<const float4*>(first + static_cast<size_t>(s) * kBM * BN + c * 32);
+                                    const float4* src = reinterpret_cast<const float4*>(first + static_cast<size_t>(s) * kBM * BN + c * 8 * (kBM * 4));
 #pragma unroll
                                     for (int v = 0; v < 8; ++v) {
-                                        const float4 a = __ldcg(src + v), b = __ldcg(src + BN / 8 + v);
+                                        const float4 a = __ldcg(src + v * kBM), b = __ldcg(src + (BN / 8 + v) * kBM);
                                         gate[4 * v] += a.x; gate[4 * v + 1] += a.y; gate[4 * v + 2] += a.z; gate[4 * v + 3] += a.w;
                                         up[4 * v] += b.x; up[4 * v + 1] += b.y; up[4 * v + 2] += b.z; up[4 * v + 3] += b.w;
                                     }
@@ -1456,10 +1462,10 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
 #pragma unroll
                             for (int i = 0; i < 32; ++i) accv[i] = 0.f;
                             for (int s = 0; s < p.splits; ++s) {
-                                const float4* src = reinterpret_cast<const float4*>(first + static_cast<size_t>(s) * kBM * BN + c * 32);
+                                const float4* src = reinterpret_cast<const float4*>(first + static_cast<size_t>(s) * kBM * BN + c * 8 * (kBM * 4));
 #pragma unroll
                                 for (int v = 0; v < 8; ++v) {
-                                    float4 t = __ldcg(src + v);
+                                    float4 t = __ldcg(src + v * kBM);
                                     accv[4 * v] += t.x; accv[4 * v + 1] += t.y; accv[4 * v + 2] += t.z; accv[4 * v + 3] += t.w;
                                 }
                             }

@@ -392,7 +392,7 @@ class Context:
         return xb, xr, xc, yc
 
     def gated_forward(self, x, w, activation="silu", out=None, pre=None, dropout=None):
-        """h = act(x w[0]) * (x w[1]) in one launch, then `dropout` (a Dropout) on h.  x [xb, xr, xc], w [2, xc, yc] (the gate and the up
+        """h = act(x w[0]) * (x w[1]), then `dropout` (a Dropout) on h, in the product's epilogue.  x [xb, xr, xc], w [2, xc, yc] (the gate and the up
         projection), h [xb, xr, yc].  pre [2, xb * xr, yc] receives both projections, which the backward pass reads; None when
         there is none to come."""
         dt = self._on_device(x, w) if pre is None else self._on_device(x, w, pre)

@@ -288,7 +288,7 @@ typedef struct d8k_dropout {
     const unsigned long long* device_offset;
 } d8k_dropout;
 
-/* pre[b] = x * w[b], b = 0, 1, and h = act(pre[0]) * pre[1], then dropout on h when drop is not NULL, in one launch.
+/* pre[b] = x * w[b], b = 0, 1, and h = act(pre[0]) * pre[1], then dropout on h when drop is not NULL, formed in the product's own epilogue.
  * x is xb matrices xr x xc whose rows are taken together, w two matrices xc x yc (gate and up projection, one tensor), h has xb * xr rows of
  * yc; pre, 2 x (xb * xr) x yc, is what the backward pass needs, or NULL.  h comes from the fp32 accumulators with one rounding.  xb * xr may be 0;
  * it, xc and yc are at most 2^30.  D8K_F32: error about 4e-7 of the products in norm (a plain fp32 product: 3e-7 to 1.6e-6); an infinite
@@ -299,10 +299,10 @@ D8K_API int d8k_gated_forward(d8k_ctx* ctx, int dtype, int activation, const voi
  * elements each (pre and dpre hold 2 n).  dpre may be pre. */
 D8K_API int d8k_gated_grad_pre(d8k_ctx* ctx, int dtype, int activation, const void* pre, const void* dz, void* dpre, size_t n,
                                const d8k_dropout* drop);
-/* dx (+)= dpre[0] * w[0]^T + dpre[1] * w[1]^T, one launch; accumulate == 0 overwrites, as in d8k_matmul_grad_x_into. */
+/* dx (+)= dpre[0] * w[0]^T + dpre[1] * w[1]^T as one contraction; accumulate == 0 overwrites, as in d8k_matmul_grad_x_into. */
 D8K_API int d8k_gated_grad_x_into(d8k_ctx* ctx, int dtype, void* dx, int xb, int xr, int xc, const void* w, int yc, const void* dpre,
                                   int accumulate);
-/* dw[b] (+)= x^T * dpre[b], one launch for both. */
+/* dw[b] (+)= x^T * dpre[b], both in one launch (and one that sums slices, where the batch is long and the weights are small). */
 D8K_API int d8k_gated_grad_w_into(d8k_ctx* ctx, int dtype, const void* x, int xb, int xr, int xc, void* dw, int yc, const void* dpre,
                                   int accumulate);
 /* The three above: dpre from pre and dz, then dx and dw; dx or dw may be NULL.  dpre (2 x rows x yc) is workspace, its contents afterwards
