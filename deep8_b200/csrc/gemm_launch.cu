@@ -653,6 +653,10 @@ int run_gemm(Ctx* ctx, const GemmProblem& g, PreparedGemm* capture) {
     return 0;
 }
 
+// The one-CTA kernels' splits in the gated block: k-blocks at least (make_plan's rule asks for 24).  fp32: dx 320 x 256 from 2 x 1024 in 18.3 us with 5
+// splits, 26.6 with 2; 333 x 250 from 2 x 1001 25.4 for 33.6; 160 x 1536 -> 2 x 512 forward 21.5 with 4, 25.9 with 2; none of 33 shapes slower.
+constexpr int kGatedSplitBlocks = 12;
+
 // How the gated block's fp16 products run: 0 on the one-CTA kernel, 1 on the paired kernel, more on the paired kernel in that many slices.
 // A model in us, from measured times.  Paired: a stage (128 k) of a 256 x 256 tile 0.76, but a tile not less than `store`, its epilogue; one-CTA: a
 // k-block of 64 on a 128 x 128 tile 0.5, whatever it multiplies, a tile not less than 2.5, and 8 more where its rows leave element by element
@@ -663,11 +667,11 @@ static int pair_slices(const Ctx* ctx, long long tiles, long long singles, int i
     const int pairs = ctx->num_sms / 2;
     auto rounds = [](long long work, int at_once) { return static_cast<double>((work + at_once - 1) / at_once); };
     auto longer = [](double a, double b) { return a > b ? a : b; };
-    // the one-CTA kernel splits, too, when its tiles leave half of the SMs idle: at least 24 k-blocks each
+    // the one-CTA kernel splits, too, when its tiles leave half of the SMs idle
     double kb = 2.0 * its, extra = 0;
     if (singles * 2 <= ctx->num_sms) {
         long long s = ctx->num_sms / singles;
-        if (s > its / 12) s = its / 12;
+        if (s > 2 * its / kGatedSplitBlocks) s = 2 * its / kGatedSplitBlocks;
         if (s > 1) {
             kb /= s;
             extra = 4;
@@ -705,6 +709,18 @@ bool gated_grad_x_wants_padded_w(const Ctx* ctx, int rows, int xc, int yc) {
     return tiles < (1LL << 30) && pair_slices(ctx, tiles, singles, 2 * ((yc + 127) / 128), 3.0, xc % 8 != 0, &gain) != 0 && gain > pad_cost(4.0 * xc * yc);
 }
 
+// run_gemm with this block's split
+static int run_one_cta(Ctx* ctx, const GemmProblem& g) {
+    GemmProblem q = g;
+    const int bn = g.dtype == 1 ? 64 : 128, bk = g.dtype == 1 ? 32 : 64;
+    const long long tiles = static_cast<long long>(g.batch) * ((g.M + 127LL) / 128) * ((g.N + bn - 1LL) / bn);
+    if (tiles * 2 <= ctx->num_sms) {
+        const int blocks = g.kbatch * ((g.K + bk - 1) / bk) / kGatedSplitBlocks, most = ctx->num_sms / static_cast<int>(tiles);
+        q.force_splits = blocks < 1 ? 1 : blocks < most ? blocks : most;
+    }
+    return run_gemm(ctx, q);
+}
+
 int run_gated_grad(Ctx* ctx, const GemmProblem& g) {
     // Whole 64-element groups of each stored row, or rows padded to them.  An MN-major operand's k are rows, which end anywhere (what a box
     // holds beyond them is zeros).
@@ -713,12 +729,12 @@ int run_gated_grad(Ctx* ctx, const GemmProblem& g) {
     const long long tiles_m = (g.M + 255LL) / 256, tiles_n = (g.N + 255LL) / 256, tiles = g.batch * tiles_m * tiles_n;
     if (g.dtype != 0 || g.a.mn != g.b.mn || !whole || !tma_ok(g.a, 2) || !tma_ok(g.b, 2) || encode_tiled() == nullptr || tiles >= (1LL << 30) ||
         !env_int("D8K_PAIR", 1) || env_int("D8K_FORCE_GATHER", 0))
-        return run_gemm(ctx, g);
+        return run_one_cta(ctx, g);
     const long long singles = static_cast<long long>(g.batch) * ((g.M + 127LL) / 128) * ((g.N + 127LL) / 128);
     const int num_kb = (g.K + 63) / 64, its = g.kbatch * ((num_kb + 1) / 2);
     const bool ragged = ((g.ldc | g.c_batch_stride) & 7) != 0 || (reinterpret_cast<uintptr_t>(g.C) & 15) != 0;
     const int slices = pair_slices(ctx, tiles, singles, its, 3.0, ragged);
-    if (slices == 0) return run_gemm(ctx, g);
+    if (slices == 0) return run_one_cta(ctx, g);
     GemmParams p;
     std::memset(&p, 0, sizeof(p));
     p.M = g.M; p.N = g.N; p.K = g.K;
@@ -896,10 +912,10 @@ int run_gated(Ctx* ctx, const GatedProblem& g) {
     p.tiles_m = static_cast<int>(pair || slices ? (g.M + 255LL) / 256 : mtiles);
     p.tiles_n = static_cast<int>(tiles / p.tiles_m);
     p.raster_group = 16;
-    int splits = 1;  // as in make_plan: at least 24 k-blocks per split
+    int splits = 1;  // as in make_plan
     if (!pair && !slices && tiles * 2 <= ctx->num_sms && tiles <= kMaxCounters) {
         splits = ctx->num_sms / static_cast<int>(tiles);
-        if (splits > p.num_kb / 24) splits = p.num_kb / 24;
+        if (splits > p.num_kb / kGatedSplitBlocks) splits = p.num_kb / kGatedSplitBlocks;
         const size_t per_split = static_cast<size_t>(tiles) * kBM * bn * sizeof(float);
         if (splits > 1 && per_split * splits > ctx->scratch_bytes) splits = static_cast<int>(ctx->scratch_bytes / per_split);
         if (splits > 255) splits = 255;
