@@ -784,6 +784,110 @@ def test_odd_rows_captured(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("sizes", [(1, 2048, 200), (5, 1024, 2048), (48, 1600, 264), (256, 4096, 512), (1000, 192, 320), (300, 1001, 2003)], ids=str)
+def test_accumulating_calls_captured(sizes, dtype):
+    """Kernels that join partial sums (in a cluster, by a last arrival, by tickets, by a second launch), captured and replayed with new inputs in
+    the same memory and gradients that grow: the bits of the eager calls."""
+    import deep8_b200
+    rows, cols, width = sizes
+    c = deep8_b200.Context(0)
+    side = torch.cuda.Stream()
+    c.use_stream(side)
+    with torch.cuda.stream(side):
+        x, w, dz = torch.empty(1, rows, cols, dtype=dtype, device=DEV), torch.empty(2, cols, width, dtype=dtype, device=DEV), tensor(3, (1, rows, width), dtype, 0.1)
+        h, pre, dpre = torch.empty_like(dz), torch.empty(2, rows, width, dtype=dtype, device=DEV), torch.empty(2, rows, width, dtype=dtype, device=DEV)
+        dx, dw = torch.zeros_like(x), torch.zeros_like(w)
+
+        def step():
+            c.gated_forward(x, w, "gelu", out=h, pre=pre)
+            c.gated_backward(x, w, pre, dz, dx, dw, "gelu", dpre=dpre)
+
+        def fill(k):
+            x.copy_(tensor(50 + k, x.shape, dtype))
+            w.copy_(tensor(60 + k, w.shape, dtype, cols ** -0.5))
+
+        wanted = []
+        for k in range(3):
+            fill(k)
+            step()
+            wanted.append([t.clone() for t in (h, pre, dx, dw)])
+        side.synchronize()
+        check_gated(x, w, "gelu", h, pre)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            step()
+        dx.zero_()
+        dw.zero_()
+        for k in range(3):
+            fill(k)
+            h.fill_(float("nan"))
+            g.replay()
+            side.synchronize()
+            for got, want in zip((h, pre, dx, dw), wanted[k]):
+                assert torch.equal(got, want), k
+    assert c.status() == 0
+    del g
+    c.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_backward_on_views_off_the_16_byte_boundary(ctx, dtype):
+    rows, cols, width = 300, 256, 520
+
+    def view(t, shift):
+        whole = torch.full((t.numel() + 8,), 7.0, dtype=dtype, device=DEV)
+        part = whole[shift:shift + t.numel()].view(t.shape)
+        return whole, part.copy_(t)
+
+    x, w = tensor(13, (1, rows, cols), dtype), tensor(14, (2, cols, width), dtype, 1.0 / 16)
+    pre, dz = tensor(15, (2, rows, width), dtype), tensor(16, (1, rows, width), dtype, 0.1)
+    zx, zw = torch.zeros_like(x), torch.zeros_like(w)
+    for place in range(8):
+        shifts = [(1 + k % 3) * (place in (k, 7)) for k in range(7)]
+        parts = [view(t, s) for t, s in zip((x, w, pre, dz, zx, zw, pre), shifts)]
+        (_, x1), (_, w1), (_, pre1), (_, dz1), (dx_all, dx), (dw_all, dw), (dpre_all, dpre) = parts
+        ctx.gated_backward(x1, w1, pre1, dz1, dx, dw, "silu", dpre=dpre, accumulate=place % 2 == 0)
+        check_backward(x, w, pre, dz, dx, dw, "silu", None)
+        for whole, part, shift in ((dx_all, dx, shifts[4]), (dw_all, dw, shifts[5]), (dpre_all, dpre, shifts[6])):
+            assert (whole[:shift] == 7).all() and (whole[shift + part.numel():] == 7).all()
+    assert ctx.status() == 0
+
+
+@pytest.mark.gpu
+def test_padding_memory_grows_while_another_stream_is_captured():
+    """Two contexts: one's call is captured while the other, on its own stream, needs more memory for its padded copies."""
+    import deep8_b200
+    a, b = deep8_b200.Context(0), deep8_b200.Context(0)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    a.use_stream(sa)
+    b.use_stream(sb)
+    x, w = tensor(1, (1, 48, 256), torch.float16), tensor(2, (2, 256, 512), torch.float16, 1.0 / 16)
+    h = a.gated_forward(x, w)
+    x1, w1 = tensor(3, (1, 40, 255), torch.float16), tensor(4, (2, 255, 511), torch.float16, 1.0 / 16)
+    small = b.gated_forward(x1, w1)
+    x2, w2 = tensor(5, (1, 40, 4095), torch.float16), tensor(6, (2, 4095, 2003), torch.float16, 1.0 / 64)  # 33 MB of copies
+    large, out = torch.empty(1, 40, 2003, dtype=torch.float16, device=DEV), torch.empty_like(h)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=sa):
+        a.gated_forward(x, w, out=out)
+        b.gated_forward(x2, w2, out=large)
+        a.dropout_forward(out, ops.Dropout(0.5, 1), out=out)
+    torch.cuda.synchronize()
+    check_gated(x1, w1, "silu", small, None)
+    check_gated(x2, w2, "silu", large, None)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, a.dropout_forward(h, ops.Dropout(0.5, 1)))
+    assert a.status() == 0 and b.status() == 0
+    del g
+    a.close()
+    b.close()
+
+
+@pytest.mark.gpu
 def test_gated_beyond_32_bit_offsets(ctx):
     """More than 2^32 elements of h: the last rows, with dropout, against the plain form."""
     rows, cols, width = 66000, 64, 66048
