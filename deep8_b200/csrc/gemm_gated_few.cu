@@ -3,7 +3,9 @@
 // The operands change places: 128 columns of a projection are the M side of the MMA (w is MN-major there), the tokens its N side, so that
 // an accumulator is 128 x (16 .. 128) instead of 128 rows of which most would be padding, a partial sum of a split contraction is
 // rows x 128 values, and a stage of shared memory is almost all weights.
-// Measured (4096 -> 2 x 16384): the ordinary gated kernels take 57 to 77 us for 8 to 64 rows, whose weights alone are 41 us of HBM time.
+// Measured (4096 -> 2 x 16384, whose weights alone are 41 us of HBM time): 44 us for 1 to 16 rows (6.1 TB/s), 47 for 48, 48 for 128; the ordinary
+// gated kernels 57 to 77 us for 8 to 64 rows.  2048 -> 2 x 5504 (6.9 us of HBM time): 14 us for up to 8 rows, 16.5 for 48, 20 for 128; there the
+// launch, the first loads and the joining of two slices take as long as the weights.
 //
 // Roles, barriers and bounded waits are those of d8k_gemm_kernel with one thread per role.  A work item is a strip of 128 columns and a
 // slice of the contraction.  Unsplit, persistent CTAs walk over the strips, the epilogue of one (two accumulator buffers) beside the main
