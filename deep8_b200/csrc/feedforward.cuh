@@ -22,7 +22,10 @@ __device__ __forceinline__ float sigmoid_of(float a) {
 }
 
 // value = act(a); slope = act'(a) when wanted.  gelu goes through erfc, gelu_tanh through a sigmoid ((1 + tanh z) / 2 = sigmoid(2 z)):
-// both forms keep the relative accuracy of the negative tail, where 1 + erf and 1 + tanh cancel.  Arguments beyond +-80 take the
+// both forms keep the relative accuracy of the negative tail, where 1 + erf and 1 + tanh cancel.  FAST: the normal distribution's tail
+// beyond |a| is exp(-a^2 / 2) q(|a|), and q a polynomial of degree 7 in 1 / (1 + 0.264 |a|) without a constant, fitted for the least largest
+// relative error over |a| <= 14 (5.8e-7; linear programming on 1200 Chebyshev points); the library's erfc made the fp16 product of
+// 1531 x 1024 by two of 1024 x 4096 a third longer than the other activations.  Arguments beyond +-80 take the
 // limits' values (an fp16 projection may have overflowed to an infinity, and infinity times a vanished factor would be a NaN).
 template <int ACT, bool FAST, bool SLOPE>
 __device__ __forceinline__ void activation(float a, float& value, float& slope) {
@@ -40,9 +43,25 @@ __device__ __forceinline__ void activation(float a, float& value, float& slope) 
         value = lo * s;
         if (SLOPE) slope = fmaf(b * s * (1.0f - s), c2 * fmaf(0.134145f, b2, 1.0f), s);
     } else if constexpr (ACT == kActGelu) {
-        const float cdf = 0.5f * erfcf(-0.7071067811865476f * b);
+        float cdf, e;
+        if constexpr (FAST) {
+            const float x = fabsf(b), t = __fdividef(1.0f, fmaf(0.26445794f, x, 1.0f));
+            e = __expf(-0.5f * b * b);
+            float q = -0.068581074f;
+            q = fmaf(q, t, 0.19961888f);
+            q = fmaf(q, t, -0.071617506f);
+            q = fmaf(q, t, 0.14575285f);
+            q = fmaf(q, t, 0.08163642f);
+            q = fmaf(q, t, 0.10782069f);
+            q = fmaf(q, t, 0.10536946f);
+            const float tail = e * (q * t);
+            cdf = b < 0.0f ? tail : 1.0f - tail;
+        } else {
+            cdf = 0.5f * erfcf(-0.7071067811865476f * b);
+            if (SLOPE) e = expf(-0.5f * b * b);
+        }
         value = lo * cdf;
-        if (SLOPE) slope = fmaf(b * 0.3989422804014327f, FAST ? __expf(-0.5f * b * b) : expf(-0.5f * b * b), cdf);
+        if (SLOPE) slope = fmaf(b * 0.3989422804014327f, e, cdf);
     } else {  // relu: a NaN gives 0, as in the framework's ReLU
         value = a > 0.0f ? a : 0.0f;
         if (SLOPE) slope = a > 0.0f ? 1.0f : 0.0f;
