@@ -404,6 +404,15 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             };
             issue_c(0);
             issue_e1(0);
+            // GATED: the dropout's decisions for this thread's row in its two chunks of columns, drawn while the main loop runs
+            uint32_t stays[2] = {0xffffffffu, 0xffffffffu};
+            if constexpr (Cfg::GATED && !Cfg::SPLIT) {
+                if (p.gated.dropping) {
+                    const unsigned long long at = static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + it.n0 / 2 + (warp < 4 ? 0 : 64);
+                    stays[0] = drop_mask32(p.gated.drop, at);
+                    stays[1] = drop_mask32(p.gated.drop, at + 32);
+                }
+            }
             const long long tw = p.prof ? clock64() : 0;
             ok = wait_bar(tfull_bar(acc), acc_phase, &s_abort, p.status, (kRoleEpilogue << 8) | 3, static_cast<unsigned>(p.epi_backoff_ns));
             if (!ok) break;
@@ -509,8 +518,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                     if (col0 >= p.N) continue;
                     const uint32_t s0 = staging, s1 = staging + Cfg::SLOT_BYTES;
                     using V = EpiVec<OutT>;
-                    const uint32_t stays =
-                        t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0) : 0xffffffffu;
+                    const uint32_t keep = stays[c - c_begin];
                     if (!segments || col0 + 32 > p.N) {
                         // rows that start anywhere, or end inside these columns: one row per store, a column per lane
                         auto rows_out = [&](OutT* dst, uint32_t slot) {
@@ -527,7 +535,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                             rows_out(reinterpret_cast<OutT*>(t.pre), 0);
                             rows_out(reinterpret_cast<OutT*>(t.pre) + t.pre_stride, Cfg::SLOT_BYTES);
                         }
-                        gated_values<OutT>(t, stays, gate, up);
+                        gated_values<OutT>(t, keep, gate, up);
 #pragma unroll
                         for (int v = 0; v < 4; ++v) st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
                         rows_out(reinterpret_cast<OutT*>(p.C), 0);
@@ -552,7 +560,7 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
                         }
                         __syncwarp();
                     }
-                    gated_values<OutT>(t, stays, gate, up);
+                    gated_values<OutT>(t, keep, gate, up);
 #pragma unroll
                     for (int v = 0; v < 4; ++v) st_shared_v4(s0 + slot_off(lane, v), V::pack(gate + 8 * v));
                     __syncwarp();
