@@ -405,13 +405,11 @@ d8k_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             issue_c(0);
             issue_e1(0);
             // GATED: the dropout's decisions for this thread's row in its two chunks of columns, drawn while the main loop runs
-            uint32_t stays[2] = {0xffffffffu, 0xffffffffu};
+            [[maybe_unused]] uint32_t stays[2];
             if constexpr (Cfg::GATED && !Cfg::SPLIT) {
-                if (p.gated.dropping) {
-                    const unsigned long long at = static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + it.n0 / 2 + (warp < 4 ? 0 : 64);
-                    stays[0] = drop_mask32(p.gated.drop, at);
-                    stays[1] = drop_mask32(p.gated.drop, at + 32);
-                }
+                const int first = it.n0 / 2 + (warp < 4 ? 0 : 64);
+                stays[0] = gated_mask(p, row, first);
+                stays[1] = gated_mask(p, row, first + 32);
             }
             const long long tw = p.prof ? clock64() : 0;
             ok = wait_bar(tfull_bar(acc), acc_phase, &s_abort, p.status, (kRoleEpilogue << 8) | 3, static_cast<unsigned>(p.epi_backoff_ns));

@@ -813,6 +813,11 @@ __device__ __forceinline__ uint32_t drop_mask32(const DropSpec& d, unsigned long
     return bits;
 }
 
+// The dropout's decisions for 32 columns from col0 on of a gated product's row
+__device__ __forceinline__ uint32_t gated_mask(const GemmParams& p, int row, int col0) {
+    return p.gated.dropping ? drop_mask32(p.gated.drop, static_cast<unsigned long long>(row) * static_cast<unsigned long long>(p.ldc) + col0) : 0xffffffffu;
+}
+
 // gate[i] = dropout(act(gate[i]) * up[i]) for 32 elements; bit i of `stays`: the dropout's decision
 template <typename OutT>
 __device__ __forceinline__ void gated_values(const GatedTail& t, uint32_t stays, float* gate, const float* up) {
@@ -856,14 +861,13 @@ __device__ __forceinline__ void store_transposed(OutT* to, long long ld, const f
 }
 
 // Tail of a gated product for a warp's 32 rows (this lane's is `row`, which may be past the last) and 32 columns [col0, col0 + 32), clipped to N: both
-// projections (when kept) and h, each rounded once.  Called by whole warps; overwrites gate and up.
+// projections (when kept) and h, each rounded once.  stays: gated_mask's bits.  Called by whole warps; overwrites gate and up.
 template <typename OutT>
-__device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, int col0, float* gate, float* up) {
+__device__ __forceinline__ void store_gated_chunk(const GemmParams& p, int row, int col0, float* gate, float* up, uint32_t stays) {
     using V = EpiVec<OutT>;
     constexpr int VEC = V::N;
     const GatedTail& t = p.gated;
     const long long off = static_cast<long long>(row) * p.ldc + col0;
-    uint32_t stays = t.dropping ? drop_mask32(t.drop, static_cast<unsigned long long>(off)) : 0xffffffffu;
     OutT* h = reinterpret_cast<OutT*>(p.C) + off;
     OutT* pre = reinterpret_cast<OutT*>(t.pre) + off;
     const bool vec_ok = col0 + 32 <= p.N && ((reinterpret_cast<uintptr_t>(p.C) | reinterpret_cast<uintptr_t>(t.pre)) & 15) == 0 && p.ldc % VEC == 0 &&
@@ -1299,6 +1303,13 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
             // A partial tile of a split contraction, read by the thread of the same row that it was written by: four columns of all rows
             // together, so that a warp's accesses are whole lines
             float* part = p.ws + static_cast<size_t>(w) * kBM * BN + row_in_tile * 4;
+            [[maybe_unused]] uint32_t stays[Cfg::GATED ? BN / 64 : 1];  // drawn while the main loop runs
+            if constexpr (Cfg::GATED) {
+                if (p.splits == 1) {
+#pragma unroll
+                    for (int c = 0; c < BN / 64; ++c) stays[c] = gated_mask(p, row, it.n0 / 2 + c * 32);
+                }
+            }
             if constexpr (Cfg::CHUNK_KB == 0) {
                 ok = wait_bar_timed(tfull_bar(acc), acc_phase, &s_abort, p.status, (kRoleEpilogue << 8) | 3, timed, &w_tfull,
                                     static_cast<unsigned>(p.epi_backoff_ns));
@@ -1307,8 +1318,12 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                 const uint32_t taddr = tmem_base + acc * Cfg::ACC_COLS + (static_cast<uint32_t>(quarter * 32) << 16);
                 if constexpr (Cfg::GATED) {
                     if (p.splits == 1) {
-#pragma unroll 1
+#pragma unroll 1  // unrolled, the code no longer fits the instruction cache (333 x 250 -> 2 x 1001 fp16: 17 us for 14)
                         for (int c = 0; c < BN / 64; ++c) {  // 32 columns of the gate and the same 32 of the up projection
+                            uint32_t keep = stays[0];
+#pragma unroll
+                            for (int k = 1; k < BN / 64; ++k)
+                                if (c == k) keep = stays[k];
                             uint32_t r[32], s[32];
                             __syncwarp();
                             ptx::tmem_ld_32x32(taddr + c * 32, r);
@@ -1321,7 +1336,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                                     gate[i] = __uint_as_float(r[i]);
                                     up[i] = __uint_as_float(s[i]);
                                 }
-                                store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, gate, up);
+                                store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, gate, up, keep);
                             }
                         }
                     }
@@ -1390,7 +1405,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                     if (p.splits == 1) {
 #pragma unroll
                         for (int c = 0; c < BN / 64; ++c)
-                            if (it.n0 / 2 + c * 32 < p.N) store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, &accv[c * 32], &accv[BN / 2 + c * 32]);
+                            if (it.n0 / 2 + c * 32 < p.N) store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, &accv[c * 32], &accv[BN / 2 + c * 32], stays[c]);
                     }
                 }
 #pragma unroll
@@ -1452,7 +1467,7 @@ d8k_gemm_kernel(const __grid_constant__ CUtensorMap tmA_launch, const __grid_con
                                         up[4 * v] += b.x; up[4 * v + 1] += b.y; up[4 * v + 2] += b.z; up[4 * v + 3] += b.w;
                                     }
                                 }
-                                store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, gate, up);
+                                store_gated_chunk<OutT>(p, row, it.n0 / 2 + c * 32, gate, up, gated_mask(p, row, it.n0 / 2 + c * 32));
                             }
                         }
 #pragma unroll 1
