@@ -888,6 +888,47 @@ def test_padding_memory_grows_while_another_stream_is_captured():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_two_contexts_on_two_streams(dtype):
+    """Each context owns its scratch memory, arrival words, tickets and padding memory: calls of two on two streams do not meet."""
+    import deep8_b200
+    held = [(deep8_b200.Context(0), torch.cuda.Stream()) for _ in range(2)]
+    for sizes in ((1, 2048, 200), (5, 1024, 2048), (48, 1600, 264), (256, 1024, 512), (100, 1001, 203)):
+        rows, cols, width = sizes
+        calls = []
+        for k, (c, stream) in enumerate(held):
+            x, w = tensor(70 + k, (1, rows, cols), dtype), tensor(80 + k, (2, cols, width), dtype, cols ** -0.5)
+            pre, dz, gain = tensor(90 + k, (2, rows, width), dtype), tensor(100 + k, (1, rows, width), dtype, 0.1), tensor(110 + k, (cols,), dtype)
+            c.use_stream(stream)
+
+            def call(c=c, x=x, w=w, pre=pre, dz=dz, gain=gain):
+                dx, dw, dgain, rstd = torch.empty_like(x), torch.empty_like(w), torch.empty_like(gain), torch.empty(x.shape[1], device=DEV)
+                n = c.rms_norm_forward(x, gain, rstd=rstd)
+                h = c.gated_forward(n, w)
+                c.gated_backward(n, w, pre, dz, dx, dw, accumulate=False)
+                dn = torch.empty_like(x)
+                c.rms_norm_backward(x, gain, rstd, dn, dgain, dx, accumulate=False)
+                return h, dx, dw, dn, dgain
+
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                alone = call()
+            torch.cuda.synchronize()
+            calls.append((call, stream, alone))
+        together = []
+        for _ in range(4):
+            for call, stream, alone in calls:
+                with torch.cuda.stream(stream):
+                    together.append((call(), alone))
+        torch.cuda.synchronize()
+        for got, want in together:
+            assert all(torch.equal(g, w) for g, w in zip(got, want)), sizes
+    for c, _ in held:
+        assert c.status() == 0
+        c.close()
+
+
+@pytest.mark.gpu
 def test_gated_beyond_32_bit_offsets(ctx):
     """More than 2^32 elements of h: the last rows, with dropout, against the plain form."""
     rows, cols, width = 66000, 64, 66048
