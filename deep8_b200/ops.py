@@ -56,19 +56,64 @@ class Dropout:
     Philox4x32-10 at the counter (i / 4, offset + counter) under `seed` is at least p * 2^32, and is then multiplied by 1 / (1 - p).
     The backward pass gives the same object (or one with the same values); calls whose masks are to differ give different
     offsets.  counter: optional int64 tensor of one element on the GPU, read when the kernel runs, so that a captured graph
-    which advances it draws a new mask at every replay."""
+    which advances it draws a new mask at every replay.  The fields may be set between calls; a call takes them as they are then."""
 
-    __slots__ = ("p", "seed", "offset", "counter", "arg")
+    __slots__ = ("_spec", "_counter")
 
     def __init__(self, p, seed, offset=0, counter=None):
-        if not 0.0 <= p <= 1.0:
+        self._spec = _lib.DropoutSpec()  # what the library reads: the fields live here and nowhere else
+        self.p, self.seed, self.offset, self.counter = p, seed, offset, counter
+
+    @property
+    def p(self):
+        return self._spec.p
+
+    @p.setter
+    def p(self, value):
+        if not 0.0 <= value <= 1.0:
             raise ValueError("dropout: p must be between 0 and 1")
-        if not (0 <= seed < 1 << 64 and 0 <= offset < 1 << 64):
+        self._spec.p = float(value)
+
+    @staticmethod
+    def _word(value):
+        if not 0 <= value < 1 << 64:
             raise ValueError("dropout: seed and offset are unsigned 64-bit integers")
-        if counter is not None and (counter.dtype != torch.int64 or counter.numel() != 1):
+        return int(value)
+
+    @property
+    def seed(self):
+        return self._spec.seed
+
+    @seed.setter
+    def seed(self, value):
+        self._spec.seed = self._word(value)
+
+    @property
+    def offset(self):
+        return self._spec.offset
+
+    @offset.setter
+    def offset(self, value):
+        self._spec.offset = self._word(value)
+
+    @property
+    def counter(self):
+        return self._counter
+
+    @counter.setter
+    def counter(self, value):
+        if value is not None and (value.dtype != torch.int64 or value.numel() != 1):
             raise ValueError("dropout: the counter is an int64 tensor of one element")
-        self.p, self.seed, self.offset, self.counter = float(p), int(seed), int(offset), counter
-        self.arg = ctypes.byref(_lib.DropoutSpec(self.p, self.seed, self.offset, counter.data_ptr() if counter is not None else None))
+        self._counter = value
+
+    @property
+    def arg(self):
+        """The d8k_dropout argument of a call: the fields as they are now (a tensor's memory may have been exchanged under it)."""
+        self._spec.device_offset = self._counter.data_ptr() if self._counter is not None else None
+        return ctypes.byref(self._spec)
+
+    def __reduce__(self):  # a copy has a structure of its own
+        return Dropout, (self.p, self.seed, self.offset, self.counter)
 
 
 class Context:

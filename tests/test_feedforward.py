@@ -8,6 +8,7 @@ off by at most 2^-19 of its magnitude (each operand is hi + lo with |lo| <= 2^-1
 dropped).  The activations are good to 2^-18 of (1 + |a|) times their size: the fast exponential is off by (2 + 1.2 |a|) * 2^-23, erfc's
 rounded argument z by 2 z^2 * 2^-24 < 2^-18 for |z| < 5.
 """
+import copy
 import math
 import os
 import subprocess
@@ -263,6 +264,54 @@ def test_tensors_of_the_host_are_refused():
         c.dropout_forward(torch.zeros(4), ops.Dropout(0.1, 1))
     with pytest.raises(ValueError):
         c.rms_norm_forward(torch.zeros(4, 8), torch.zeros(8))
+
+
+class _RecordingLib:
+    """Stands in for the library: keeps what the dropout argument of a call points at."""
+
+    def d8k_dropout_forward(self, h, dtype, x, residual, y, n, drop):
+        spec = drop._obj
+        self.got = (spec.p, spec.seed, spec.offset, spec.device_offset)
+        return 0
+
+
+def test_dropout_fields_set_after_construction_reach_the_library(bare):
+    """A training loop that advances the offset (or exchanges the counter) gets another mask; what a constructor refuses a setter does, too."""
+    bare.lib = _RecordingLib()
+    x, top = torch.zeros(4), (1 << 64) - 1
+    first, second = torch.zeros(1, dtype=torch.int64), torch.zeros(1, dtype=torch.int64)
+    drop = ops.Dropout(0.1, 5)
+
+    def handed():
+        bare.dropout_forward(x, drop)
+        assert (drop.p, drop.seed, drop.offset) == bare.lib.got[:3]
+        return bare.lib.got
+
+    bare._device = torch.device("cpu")  # where this test's counters are
+    assert handed() == (0.1, 5, 0, None)
+    drop.offset += 1
+    drop.seed = top
+    drop.p = 0.5
+    assert handed() == (0.5, top, 1, None)
+    for counter in (first, second):
+        drop.counter = counter
+        assert drop.counter is counter and handed() == (0.5, top, 1, counter.data_ptr())
+    second.set_(torch.zeros(1, dtype=torch.int64))  # the same tensor over other memory
+    assert handed()[3] == second.data_ptr()
+    drop.counter = None
+    assert handed() == (0.5, top, 1, None)
+    for field, value in (("p", 1.5), ("p", -0.1), ("p", float("nan")), ("seed", -1), ("seed", 1 << 64), ("offset", 1 << 64),
+                         ("counter", torch.zeros(1)), ("counter", torch.zeros(2, dtype=torch.int64))):
+        with pytest.raises(ValueError):
+            setattr(drop, field, value)
+    assert handed() == (0.5, top, 1, None)
+    drop.counter = first
+    bare._device = torch.device("cuda", 0)
+    with pytest.raises(ValueError):
+        bare.dropout_forward(x, drop)  # the counter that is set now is checked, not the constructor's
+    twin = copy.copy(drop)
+    twin.offset, twin.counter = 7, None
+    assert (drop.offset, drop.counter) == (1, first) and (twin.p, twin.seed, twin.offset, twin.counter) == (0.5, top, 7, None)
 
 
 def test_library_refuses_a_null_context():
