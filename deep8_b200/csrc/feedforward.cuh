@@ -13,24 +13,30 @@ namespace d8k {
 enum : int { kActSilu = 0, kActGelu = 1, kActGeluTanh = 2, kActRelu = 3, kActSigmoid = 4, kActCount = 5 };
 
 // 1 / (1 + exp(-a)).  FAST (results that are rounded to fp16, whose step is 2^-11): the hardware exponential and a division
-// without the last rounding, a few 2^-22 together; otherwise the library's exponential and an IEEE division.
+// without the last rounding, a few 2^-22 together; 0 below -80, where exp(80) keeps the division in its full range and under 2^-115 is
+// nothing beside fp16's 2^-25.  Otherwise the library's exponential and an IEEE division, for negative arguments as e / (1 + e) with
+// e = exp(a), which follows the result down to the smallest floats (1 / (1 + exp(-a)) would lose it where exp(-a) overflows).
 template <bool FAST>
 __device__ __forceinline__ float sigmoid_of(float a) {
-    if (a < -80.0f) return 0.0f;  // under 2^-115; exp(80) keeps both divisions in their full range
-    if constexpr (FAST) return __fdividef(1.0f, 1.0f + __expf(-a));
-    else return 1.0f / (1.0f + expf(-a));
+    if constexpr (FAST) {
+        if (a < -80.0f) return 0.0f;
+        return __fdividef(1.0f, 1.0f + __expf(-a));
+    } else {
+        const float e = expf(-fabsf(a)), r = 1.0f / (1.0f + e);
+        return a < 0.0f ? e * r : r;
+    }
 }
 
 // value = act(a); slope = act'(a) when wanted.  gelu goes through erfc, gelu_tanh through a sigmoid ((1 + tanh z) / 2 = sigmoid(2 z)):
 // both forms keep the relative accuracy of the negative tail, where 1 + erf and 1 + tanh cancel.  FAST: the normal distribution's tail
 // beyond |a| is exp(-a^2 / 2) q(|a|), and q a polynomial of degree 7 in 1 / (1 + 0.264 |a|) without a constant, fitted for the least largest
 // relative error over |a| <= 14 (5.8e-7; linear programming on 1200 Chebyshev points); the library's erfc made the fp16 product of
-// 1531 x 1024 by two of 1024 x 4096 a third longer than the other activations.  Arguments beyond +-80 take the
-// limits' values (an fp16 projection may have overflowed to an infinity, and infinity times a vanished factor would be a NaN).
+// 1531 x 1024 by two of 1024 x 4096 a third longer than the other activations.  Factors beyond +-110 count as 110 where what they multiply has
+// vanished (exp(-104) is below the smallest float; an infinite projection times a vanished factor would be a NaN).
 template <int ACT, bool FAST, bool SLOPE>
 __device__ __forceinline__ void activation(float a, float& value, float& slope) {
-    const float lo = a < -80.0f ? -80.0f : a;
-    const float b = lo > 80.0f ? 80.0f : lo;
+    const float lo = a < -110.0f ? -110.0f : a;
+    const float b = lo > 110.0f ? 110.0f : lo;
     if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
         const float s = sigmoid_of<FAST>(a);
         const float ds = s * (1.0f - s);

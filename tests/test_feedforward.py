@@ -998,6 +998,24 @@ def test_gated_beyond_32_bit_offsets(ctx):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", ["sigmoid", "silu"])
+def test_gates_far_below_zero(ctx, name):
+    """fp32 gates between -87 and -64, whose sigmoids are small but normal numbers, times an up projection of 2^100.  Gates of ten bits: their
+    products with 1 and 2^100 are exact.  The exponential is off by 2^-22, at most four operations and four more of the product by 2^-24."""
+    a = torch.arange(-87.0, -64.0, 0.125, dtype=torch.float64)
+    w = torch.tensor([1.0, 2.0 ** 100], device=DEV).view(2, 1, 1).repeat(1, 1, 4)
+    for rows in (a.numel(), 5):  # the tensor cores, the streaming kernel
+        x = a[:rows].float().to(DEV).view(1, rows, 1)
+        h64 = gated64(x[0].double(), w.double(), name)[0]
+        within(ctx.gated_forward(x, w, name)[0], h64, stored(h64, h64.abs() * 2.0 ** -21, torch.float32), "h")
+    gate = x.new_tensor(a.tolist()).view(1, 1, -1)
+    pre, dz = torch.cat((gate, torch.full_like(gate, 2.0 ** 100))), torch.ones_like(gate)
+    value, slope = act64(name, gate[0].double())
+    want = torch.stack((slope * 2.0 ** 100, value))
+    within(ctx.gated_grad_pre(pre, dz, name), want, stored(want, want.abs() * 2.0 ** -20, torch.float32), "dpre")
+
+
+@pytest.mark.gpu
 def test_cpp_nodes():
     """The C++ nodes (tests/cpp/test_feedforward_host.cu): the block as a graph, forward and backward walk."""
     exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "test_feedforward_host")
