@@ -26,6 +26,15 @@ __device__ __forceinline__ float sigmoid_of(float a) {
         return a < 0.0f ? e * r : r;
     }
 }
+// s = 1 / (1 + exp(-a)) and c = 1 - s, both to a few steps of themselves: 1 / (1 + e) and e / (1 + e) with e = exp(-|a|).  Formed as 1 - s, c would
+// be off by the spacing of floats around 1 (0.9 % of it at a = 12) and 0 from a = 17 on.
+template <bool FAST>
+__device__ __forceinline__ void sigmoid_and_rest(float a, float& s, float& c) {
+    const float e = FAST ? __expf(-fabsf(a)) : expf(-fabsf(a));
+    const float large = FAST ? __fdividef(1.0f, 1.0f + e) : 1.0f / (1.0f + e), small = e * large;
+    s = a < 0.0f ? small : large;
+    c = a < 0.0f ? large : small;
+}
 
 // value = act(a); slope = act'(a) when wanted.  gelu goes through erfc, gelu_tanh through a sigmoid ((1 + tanh z) / 2 = sigmoid(2 z)):
 // both forms keep the relative accuracy of the negative tail, where 1 + erf and 1 + tanh cancel.  FAST: the normal distribution's tail
@@ -38,16 +47,19 @@ __device__ __forceinline__ void activation(float a, float& value, float& slope) 
     const float lo = a < -110.0f ? -110.0f : a;
     const float b = lo > 110.0f ? 110.0f : lo;
     if constexpr (ACT == kActSilu || ACT == kActSigmoid) {
-        const float s = sigmoid_of<FAST>(a);
-        const float ds = s * (1.0f - s);
+        float s, c = 0.0f;
+        if constexpr (SLOPE) sigmoid_and_rest<FAST>(a, s, c);
+        else s = sigmoid_of<FAST>(a);
         value = ACT == kActSilu ? lo * s : s;
-        if (SLOPE) slope = ACT == kActSilu ? fmaf(b, ds, s) : ds;
+        if (SLOPE) slope = ACT == kActSilu ? fmaf(b * s, c, s) : s * c;
     } else if constexpr (ACT == kActGeluTanh) {
         const float c2 = 1.5957691216057308f;  // 2 sqrt(2 / pi)
-        const float b2 = b * b;
-        const float s = sigmoid_of<FAST>(c2 * b * fmaf(0.044715f, b2, 1.0f));
+        const float b2 = b * b, z = c2 * b * fmaf(0.044715f, b2, 1.0f);
+        float s, c = 0.0f;
+        if constexpr (SLOPE) sigmoid_and_rest<FAST>(z, s, c);
+        else s = sigmoid_of<FAST>(z);
         value = lo * s;
-        if (SLOPE) slope = fmaf(b * s * (1.0f - s), c2 * fmaf(0.134145f, b2, 1.0f), s);
+        if (SLOPE) slope = fmaf(b * s * c, c2 * fmaf(0.134145f, b2, 1.0f), s);
     } else if constexpr (ACT == kActGelu) {
         float cdf, e;
         if constexpr (FAST) {

@@ -1015,6 +1015,35 @@ def test_gates_far_below_zero(ctx, name):
     within(ctx.gated_grad_pre(pre, dz, name), want, stored(want, want.abs() * 2.0 ** -20, torch.float32), "dpre")
 
 
+def _slopes64(name, dtype, limit):
+    """Gates on both sides from 3 to `limit`, the plain form's slopes, and how far a slope may be off, relative to it.  One exponential e is off
+    by 2^-22 (fp32) or (2 + 1.2 |z|) 2^-23 (the fast one of fp16), enters s (1 - s) = e / (1 + e)^2 at most twice, beside at most four
+    divisions and products of 2^-22 (fast) each.  silu and gelu_tanh: z is the gate or gelu_tanh's polynomial in it, whose own
+    rounding moves the exponential by |z| 2^-22; outside +-3 their two terms cancel to no less than a third of their sizes."""
+    a = torch.linspace(3.0, limit, 4001, dtype=torch.float64).to(dtype)
+    a = torch.cat((a, -a)).to(DEV)
+    a64 = a.double()
+    slope = act64(name, a64)[1]
+    z = a64.abs() if name != "gelu_tanh" else 2 * math.sqrt(2 / math.pi) * (a64.abs() + 0.044715 * a64.abs() ** 3)
+    e = 2 * (2.0 ** -22 if dtype == torch.float32 else (2 + 1.2 * z) * 2.0 ** -23) + 4 * 2.0 ** -22
+    if name != "sigmoid":
+        e = 3 * (e + (2 * z * 2.0 ** -22 if name == "gelu_tanh" else 0.0))
+    return a, slope, e
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["sigmoid", "silu", "gelu_tanh"])
+def test_gradients_of_saturated_gates(ctx, name, dtype):
+    """act' relative to itself where 1 - sigmoid(a) is far below the spacing of floats around 1."""
+    a, slope, e = _slopes64(name, dtype, 30.0 if dtype == torch.float32 else 16.0)
+    factor = 512.0 if name == "sigmoid" else 1.0  # keeps fp16's dpre normal
+    pre = torch.stack((a, torch.full_like(a, factor))).view(2, 1, -1)
+    got = ctx.gated_grad_pre(pre, torch.full_like(pre[:1], factor), name)
+    want = slope * factor * factor
+    within(got[0, 0], want, stored(want, want.abs() * (e + 2.0 ** -23), dtype), name)
+
+
 @pytest.mark.gpu
 def test_cpp_nodes():
     """The C++ nodes (tests/cpp/test_feedforward_host.cu): the block as a graph, forward and backward walk."""
