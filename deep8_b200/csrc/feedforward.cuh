@@ -80,8 +80,8 @@ __device__ __forceinline__ void activation(float a, float& value, float& slope) 
         }
         value = lo * cdf;
         if (SLOPE) slope = fmaf(b * 0.3989422804014327f, e, cdf);
-    } else {  // relu: a NaN gives 0, as in the framework's ReLU
-        value = a > 0.0f ? a : 0.0f;
+    } else {  // relu: a NaN stays one, so that a diverged projection shows
+        value = a <= 0.0f ? 0.0f : a;
         if (SLOPE) slope = a > 0.0f ? 1.0f : 0.0f;
     }
 }

@@ -274,7 +274,7 @@ D8K_API int d8k_sum_shards_adam(d8k_ctx* ctx, int dtype, void* grad_out, const v
 #define D8K_ACT_SILU 0      /* a / (1 + exp(-a)) */
 #define D8K_ACT_GELU 1      /* a * (1 + erf(a / sqrt(2))) / 2 */
 #define D8K_ACT_GELU_TANH 2 /* a * (1 + tanh(sqrt(2 / pi) * (a + 0.044715 a^3))) / 2 */
-#define D8K_ACT_RELU 3      /* max(a, 0) */
+#define D8K_ACT_RELU 3      /* max(a, 0), and NaN for NaN as the others; the slope at 0 and at NaN is 0 */
 #define D8K_ACT_SIGMOID 4   /* 1 / (1 + exp(-a)) */
 
 /* A dropout mask, which is never stored: element i (flat index in its tensor) stays when word i % 4 of Philox4x32-10 at the counter

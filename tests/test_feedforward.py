@@ -1045,6 +1045,22 @@ def test_gradients_of_saturated_gates(ctx, name, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ACTS)
+def test_a_nan_gate_stays_visible(ctx, name, dtype):
+    """A NaN among the gate's weights makes that column of h NaN whatever the activation, and its gradients of the up projection."""
+    for rows in (1, 6, 40, 300):
+        x, w = tensor(51, (1, rows, 64), dtype), tensor(52, (2, 64, 72), dtype, 0.1)
+        w[0, 5, 3] = float("nan")
+        pre = torch.empty(2, rows, 72, dtype=dtype, device=DEV)
+        h = ctx.gated_forward(x, w, name, pre=pre)
+        column = torch.arange(72, device=DEV) == 3
+        assert torch.equal(torch.isnan(h[0]), column.expand(rows, 72)) and not torch.isnan(pre[1]).any()
+        dpre = ctx.gated_grad_pre(pre, torch.ones_like(h), name)
+        assert torch.equal(torch.isnan(dpre[1]), column.expand(rows, 72))
+
+
+@pytest.mark.gpu
 def test_cpp_nodes():
     """The C++ nodes (tests/cpp/test_feedforward_host.cu): the block as a graph, forward and backward walk."""
     exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "test_feedforward_host")
