@@ -826,13 +826,17 @@ int gated_operands(d8k_ctx* ctx, int dtype, GatedOperands* o, const void* x, con
         long long rows;
         int cols;
     } parts[3] = {{&o->x, rows, xc}, {&o->w, 2LL * xc, yc}, {&o->dpre, 2LL * rows, yc}};
+    const bool dpre_whole = yc % piece == 0 || dpre_to_come || !rows_aligned(dpre, yc, dtype);
     size_t bytes = 0, at[3] = {};
     bool wanted[3] = {};
     for (int k = 0; k < 3; ++k) {
         // Rows of whole 128-byte pieces as well where that lets a faster kernel read them: x (a small copy) for the paired kernel or, in fp32, any TMA
-        // kernel; dpre for the same when it costs no copy, in fp32 always; w where the paired kernel saves more than the copy costs.
+        // kernel; dpre for the same when it costs no copy, in fp32 always; w where the paired kernel saves more than the copy costs.  The paired
+        // kernel is fp16's, and out of the question for x and w while dpre's rows are neither whole pieces nor copied.
         const bool whole = parts[k].cols % piece == 0;
-        const bool useful = !whole && (k == 0 || (k == 1 ? dtype == D8K_F16 && gated_grad_x_wants_padded_w(ctx, rows, xc, yc) : dpre_to_come || dtype == D8K_F32));
+        const bool useful = !whole && (k == 0   ? dtype == D8K_F32 || dpre_whole
+                                       : k == 1 ? dtype == D8K_F16 && dpre_whole && gated_grad_x_wants_padded_w(ctx, rows, xc, yc)
+                                                : dpre_to_come || dtype == D8K_F32);
         wanted[k] = parts[k].o->ptr && (useful || !rows_aligned(parts[k].o->ptr, parts[k].cols, dtype));
         at[k] = bytes;
         if (wanted[k]) bytes += (static_cast<size_t>(parts[k].rows) * ((parts[k].cols + piece - 1) / piece * piece) * esize(dtype) + 255) & ~static_cast<size_t>(255);

@@ -1061,6 +1061,41 @@ def test_a_nan_gate_stays_visible(ctx, name, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("accumulate", [0, 1])
+@pytest.mark.parametrize("sizes", [(700, 512, 520), (2000, 1024, 1000), (333, 250, 1001), (300, 256, 512), (64, 72, 4104), (1500, 250, 2056),
+                                   (4096, 1024, 1000)], ids=str)
+def test_gradient_products_by_themselves(ctx, sizes, accumulate, dtype):
+    """d8k_gated_grad_x_into and d8k_gated_grad_w_into, which take dpre as it lies in the caller's memory."""
+    lib, p = _lib.load(), ops._p
+    rows, xc, yc = sizes
+    x, w, dpre = tensor(61, (1, rows, xc), dtype), tensor(62, (2, xc, yc), dtype, yc ** -0.5), tensor(63, (2, rows, yc), dtype)
+    dx0, dw0 = tensor(64, (1, rows, xc), dtype), tensor(65, (2, xc, yc), dtype)
+    dx, dw, kept = dx0.clone(), dw0.clone(), dpre.clone()
+    code = 0 if dtype == torch.float16 else 1
+    before = ctx.launch_count()
+    assert lib.d8k_gated_grad_x_into(ctx.h, code, p(dx), 1, rows, xc, p(w), yc, p(dpre), accumulate) == 0
+    # yc: rows that TMA reads as they are, but no whole 128-byte pieces.  Without a padded dpre the paired kernel, for which w or x would be copied
+    # with padding, cannot run.
+    copies_in_vain = dtype == torch.float16 and yc % 8 == 0 and yc % 64 != 0
+    if copies_in_vain:
+        assert ctx.launch_count() - before == 1
+    before = ctx.launch_count()
+    assert lib.d8k_gated_grad_w_into(ctx.h, code, p(x), 1, rows, xc, p(dw), yc, p(dpre), accumulate) == 0
+    if copies_in_vain and xc % 8 == 0:
+        assert ctx.launch_count() - before == 1
+    x64, w64, d64 = x[0].double(), w.double(), dpre.double()
+    for got, want, size, n, old in ((dx[0], torch.matmul(d64, w64.transpose(1, 2)).sum(0), torch.matmul(d64.abs(), w64.abs().transpose(1, 2)).sum(0), 2 * yc, dx0[0]),
+                                    (dw, torch.matmul(x64.t(), d64), torch.matmul(x64.abs().t(), d64.abs()), rows, dw0)):
+        err = size * (PRODUCT[dtype] + n * 2.0 ** -23)
+        if accumulate:
+            want = want + old.double()
+            err = err + want.abs() * 2.0 ** -23
+        within(got, want, stored(want, err, dtype))
+    assert torch.equal(dpre, kept) and ctx.status() == 0
+
+
+@pytest.mark.gpu
 def test_cpp_nodes():
     """The C++ nodes (tests/cpp/test_feedforward_host.cu): the block as a graph, forward and backward walk."""
     exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "test_feedforward_host")
