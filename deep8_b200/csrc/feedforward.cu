@@ -1157,7 +1157,7 @@ int d8k_gated_backward(d8k_ctx* ctx, int dtype, int activation, const void* x, i
         GatedOperands o;
         if (int rc = gated_operands(ctx, dtype, &o, dw ? x : nullptr, dx ? w : nullptr, dpre, rows, xc, yc, true)) return rc;
         void* where = const_cast<void*>(o.dpre.ptr);
-        if (o.dpre.padded)  // the zeros behind each row
+        if (o.dpre.padded && o.dpre.ld > yc)  // the zeros behind each row
             D8K_CUDA(cudaMemset2DAsync(static_cast<char*>(where) + es * yc, es * o.dpre.ld, 0, es * (o.dpre.ld - yc), 2 * static_cast<size_t>(rows), ctx->stream));
         if (int rc = gated_grad_pre(ctx, dtype, activation, pre, dz, where, static_cast<size_t>(rows) * yc, yc, static_cast<size_t>(o.dpre.ld), drop)) return rc;
         if (dx)

@@ -1096,6 +1096,37 @@ def test_gradient_products_by_themselves(ctx, sizes, accumulate, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gated_backward_with_shifted_workspace_of_whole_pieces(dtype):
+    """A workspace off the 16-byte boundary whose rows are whole 128-byte pieces: the copy's rows have nothing behind them to clear.  Eagerly and
+    captured."""
+    import deep8_b200
+    c, side = deep8_b200.Context(0), torch.cuda.Stream()
+    c.use_stream(side)
+    rows, cols, width = 40, 96, 192
+    with torch.cuda.stream(side):
+        x, w = tensor(1, (1, rows, cols), dtype), tensor(2, (2, cols, width), dtype, 0.1)
+        pre, dz = tensor(3, (2, rows, width), dtype), tensor(4, (1, rows, width), dtype, 0.1)
+        whole = torch.full((pre.numel() + 8,), 7.0, dtype=dtype, device=DEV)
+        dpre, dx, dw = whole[1:1 + pre.numel()].view(pre.shape), torch.empty_like(x), torch.empty_like(w)
+        step = lambda: c.gated_backward(x, w, pre, dz, dx, dw, "silu", dpre=dpre, accumulate=False)
+        step()
+        check_backward(x, w, pre, dz, dx, dw, "silu", None)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            step()
+        dx.fill_(float("nan"))
+        dw.fill_(float("nan"))
+        g.replay()
+        check_backward(x, w, pre, dz, dx, dw, "silu", None)
+        assert whole[0] == 7 and (whole[1 + pre.numel():] == 7).all()
+    assert c.status() == 0
+    del g
+    c.close()
+
+
+@pytest.mark.gpu
 def test_cpp_nodes():
     """The C++ nodes (tests/cpp/test_feedforward_host.cu): the block as a graph, forward and backward walk."""
     exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "test_feedforward_host")
