@@ -632,6 +632,7 @@ void checkGated(const Tensor& x, const Tensor& w, const Tensor& y) {
     DEEP8_ARGUMENT_CHECK(x.elementType == w.elementType && x.elementType == y.elementType, "the data type must be same");
     DEEP8_ARGUMENT_CHECK(2 == w.batch() && w.row() == x.col() && y.batch() == x.batch() && y.row() == x.row() && y.col() == w.col(), "the shape is error");
 }
+bool alike(const Tensor& a, const Tensor& b) { return a.shape == b.shape && a.elementType == b.elementType && a.device() == b.device(); }
 // rows of the last dimension, which `weight` matches
 size_t normRows(const Tensor& x, const Tensor& weight) {
     DEEP8_ARGUMENT_CHECK(x.device() == weight.device() && x.elementType == weight.elementType, "the device and data type must be same");
@@ -649,9 +650,7 @@ void GatedProduct(const Tensor& x, const Tensor& w, Activation activation, const
 void GatedProductGrad(const Tensor& x, Tensor* dx, const Tensor& w, Tensor* dw, Activation activation, const DropoutMask& mask, const void* pre, void* dpre,
                       const Tensor& dy, bool accumulateDx, bool accumulateDw) {
     checkGated(x, w, dy);
-    DEEP8_ARGUMENT_CHECK((nullptr == dx || (dx->shape == x.shape && dx->elementType == x.elementType)) &&
-                             (nullptr == dw || (dw->shape == w.shape && dw->elementType == w.elementType)),
-                         "the shape or type is error");
+    DEEP8_ARGUMENT_CHECK((nullptr == dx || alike(*dx, x)) && (nullptr == dw || alike(*dw, w)), "the shape, type or device is error");
     const d8k_dropout drop = maskOf(mask);
     d8k_ctx* kernels = gpuOf(x)->kernels;
     const int type = d8kType(x), batch = (int)x.batch(), row = (int)x.row(), col = (int)x.col(), width = (int)w.col();
@@ -683,7 +682,7 @@ void RMSNorm(const Tensor& x, const Tensor& weight, float epsilon, float* rstd, 
 }
 void RMSNormGrad(const Tensor& x, Tensor* dx, const Tensor& weight, Tensor* dweight, const float* rstd, const Tensor& dy, bool accumulateDx,
                  bool accumulateDweight) {
-    DEEP8_ARGUMENT_CHECK(x.shape == dy.shape && (nullptr == dx || dx->shape == x.shape) && (nullptr == dweight || dweight->shape == weight.shape), "the shape is error");
+    DEEP8_ARGUMENT_CHECK(alike(dy, x) && (nullptr == dx || alike(*dx, x)) && (nullptr == dweight || alike(*dweight, weight)), "the shape, type or device is error");
     const size_t rows = normRows(x, weight);
     auto run = [&](Tensor* a, Tensor* b, bool accumulate) {
         d8kCheck(d8k_rms_norm_backward(gpuOf(x)->kernels, d8kType(x), x.raw(), weight.raw(), rstd, a ? a->raw() : nullptr, b ? b->raw() : nullptr, dy.raw(), rows,

@@ -322,6 +322,14 @@ def test_library_refuses_a_null_context():
     assert b"context" in lib.d8k_last_error()
 
 
+def test_cpp_gradient_checks():
+    """What the C++ gradients refuse before they touch a device (tests/cpp/test_feedforward_checks.cu)."""
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "test_feedforward_checks")
+    assert os.path.exists(exe), "tests/cpp/bin/test_feedforward_checks is missing: run __graft_entry__.build()"
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
