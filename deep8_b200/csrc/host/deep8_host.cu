@@ -1289,6 +1289,32 @@ void bfs(Node* last, F visit) {
             if (seen.insert(in).second) que.push(in);
     }
 }
+
+// The backward walk's order: the queue order wherever it visits every node behind all that read it, as it does in chains and in graphs whose
+// paths between two nodes are equally long - bit for bit the reference's sums there.  Where a path is shorter (a residual stream that
+// the next block and the addition behind it read), the queue reaches a producer before the longer path has added to its gradient, and that
+// part would be lost: then a node waits in the queue until the last of its readers has been visited.
+std::vector<Node*> backwardOrder(Node* last) {
+    std::vector<Node*> order;
+    std::unordered_map<Node*, size_t> readers;  // inputs of visited nodes that name it and have not been visited
+    bfs(last, [&](Node* n) {
+        order.push_back(n);
+        for (auto in : n->inputs) ++readers[in];
+    });
+    auto left = readers;
+    bool ordered = true;
+    for (auto n : order) {
+        auto it = left.find(n);
+        ordered = ordered && (it == left.end() || 0 == it->second);
+        for (auto in : n->inputs) --left[in];
+    }
+    if (ordered) return order;
+    order.assign(1, last);
+    for (size_t i = 0; i < order.size(); ++i)
+        for (auto in : order[i]->inputs)
+            if (0 == --readers[in]) order.push_back(in);
+    return order;
+}
 }  // namespace
 
 void EagerExecutor::backward(Node* last, bool clearInterim) {
@@ -1359,7 +1385,7 @@ void EagerExecutor::backwardFrom(Variable* last, const void* hostGradient, const
         last->gradientTouched = true;
     }
     std::unordered_set<Node*> done;
-    bfs(last, [this, &done](Node* n) { backwardNode(n, done); });
+    for (auto n : backwardOrder(last)) backwardNode(n, done);
     if (touch)
         bfs(last, [](Node* n) {  // a gradient nothing contributed to reads as zeros, as after the reference's zero fill
             if (NodeType::Variable != n->type) return;

@@ -618,7 +618,8 @@ public:
     explicit EagerExecutor(DeviceType deviceType = DeviceType::GPU, int deviceId = 0);
     Variable* addFunction(Function* func) override;
     void forward(Node* last) override;
-    // the reference's rule: `last` must be a scalar Variable; its gradient is set to one
+    // the reference's rule: `last` must be a scalar Variable; its gradient is set to one.  The walk takes the reference's queue order (breadth
+    // first) unless that visits a node before all that read it, which the reference lets lose gradients; then a node waits for its readers
     void backward(Node* last, bool clearInterim = true) override;
     // addition: start from `last` with an upstream gradient given on the host (the benchmark configurations supply one)
     void backward(Variable* last, const void* hostGradient, bool clearInterim = true);

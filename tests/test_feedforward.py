@@ -1141,3 +1141,12 @@ def test_cpp_nodes():
     assert os.path.exists(exe), "tests/cpp/bin/test_feedforward_host is missing: run __graft_entry__.build()"
     r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
+
+
+@pytest.mark.gpu
+def test_cpp_node_graphs():
+    """Graphs of several blocks and shared variables, both types, every activation (tests/cpp/test_feedforward_nodes.cu)."""
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "bin", "test_feedforward_nodes")
+    assert os.path.exists(exe), "tests/cpp/bin/test_feedforward_nodes is missing: run __graft_entry__.build()"
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
