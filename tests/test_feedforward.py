@@ -330,6 +330,34 @@ def test_cpp_gradient_checks():
     assert r.returncode == 0, r.stdout + r.stderr
 
 
+def _philox_raw(counter, key):
+    """Philox4x32-10 of one 128-bit counter under a 64-bit key, lists of 32-bit words, lowest first, in Python's integers."""
+    c, k = list(counter), list(key)
+    for _ in range(10):
+        a, b = 0xD2511F53 * c[0], 0xCD9E8D57 * c[2]
+        c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+# counter, key, words: the generator's published answers (the authors' Random123 distribution, its known-answer list for philox4x32 10)
+PHILOX_ANSWERS = [([0] * 4, [0] * 2, [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]),
+                  ([0xffffffff] * 4, [0xffffffff] * 2, [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]),
+                  ([0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344], [0xa4093822, 0x299f31d0], [0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1])]
+
+
+def test_generator_published_answers():
+    """All three published vectors, and the plain generator of this file against them where its element index can reach the counter: the words
+    of seed and offset have a place of their own each."""
+    for counter, key, words in PHILOX_ANSWERS:
+        assert _philox_raw(counter, key) == words
+    seed, offset, group = 0x299f31d0a4093822, 0x0370734413198a2e, 0x05a308d3243f6a88
+    want = _philox_raw([group & 0xFFFFFFFF, group >> 32, offset & 0xFFFFFFFF, offset >> 32], [seed & 0xFFFFFFFF, seed >> 32])
+    assert [int(v) for v in philox_words(seed, offset, 4 * group, 4)] == want
+    counter, key, words = PHILOX_ANSWERS[2]
+    assert [int(v) for v in philox_words(key[0] | key[1] << 32, counter[2] | counter[3] << 32, 8, 1)] == _philox_raw([2, 0] + counter[2:], key)[:1]
+
+
 # ------------------------------------------------------------------------------------------------ on the GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
@@ -1131,6 +1159,65 @@ def test_gated_backward_with_shifted_workspace_of_whole_pieces(dtype):
         assert whole[0] == 7 and (whole[1 + pre.numel():] == 7).all()
     assert c.status() == 0
     del g
+    c.close()
+
+
+@pytest.mark.gpu
+def test_device_generator_against_raw_counters(ctx):
+    """The device's decisions for the first groups, bit by bit: with p = 1/2 an element stays when its word's top bit is set; p = 2^-k masks the
+    bits further down."""
+    seed, offset = 0x299f31d0a4093822, 0x0370734413198a2e
+    words = [w for group in range(64) for w in _philox_raw([group, 0, offset & 0xFFFFFFFF, offset >> 32], [seed & 0xFFFFFFFF, seed >> 32])]
+    for p in (0.5, 0.25, 1.0 / 3, 0.9, 2.0 ** -32, 1.0 - 2.0 ** -32):
+        y = ctx.dropout_forward(torch.ones(256, device=DEV), ops.Dropout(p, seed, offset))
+        assert [bool(v) for v in (y != 0).tolist()] == [w >= round(p * 2 ** 32) for w in words], p
+
+
+@pytest.mark.gpu
+def test_dropout_beyond_the_counters_low_word():
+    """2^34 elements and more: their groups no longer fit the counter's first word, and a second launch takes them.  In place, 34 GB."""
+    import deep8_b200
+    n = (1 << 34) + 4099
+    if torch.cuda.mem_get_info()[0] < 2 * n + (2 << 30):
+        pytest.skip("needs 36 GB of device memory")
+    c = deep8_b200.Context(0)
+    x = torch.ones(n, dtype=torch.float16, device=DEV)
+    drop = ops.Dropout(0.5, 17, 3)
+    c.dropout_forward(x, drop, out=x)
+    for first, count in ((0, 4000), ((1 << 34) - 100, 4099), (n - 3, 3)):
+        assert torch.equal(x[first:first + count], keep_mask(drop, (count,), first).to(DEV).half() * 2), first
+    c.close()
+    del x
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scratch", [4096, 1 << 20])
+def test_contexts_with_little_scratch_memory(scratch, dtype):
+    """Plans that would split a contraction have to do with what the context was given."""
+    import deep8_b200
+    c = deep8_b200.Context(0, scratch)
+    for rows, xc, yc in ((1, 4096, 512), (7, 2048, 1032), (48, 1600, 264), (127, 1000, 504), (300, 512, 520), (256, 4096, 128), (700, 512, 2048)):
+        x, w = tensor(1, (1, rows, xc), dtype), tensor(2, (2, xc, yc), dtype, xc ** -0.5)
+        pre = torch.empty(2, rows, yc, dtype=dtype, device=DEV)
+        h = c.gated_forward(x, w, "silu", pre=pre)
+        check_gated(x, w, "silu", h, pre)
+        pre, dz = tensor(3, (2, rows, yc), dtype), tensor(4, (1, rows, yc), dtype, 0.1)
+        dx, dw = torch.empty_like(x), torch.empty_like(w)
+        c.gated_backward(x, w, pre, dz, dx, dw, "silu", accumulate=False)
+        check_backward(x, w, pre, dz, dx, dw, "silu", None)
+    rows, cols = 600, 1000
+    x, weight, dy, rstd = tensor(5, (rows, cols), dtype), tensor(6, (cols,), dtype), tensor(7, (rows, cols), dtype), torch.empty(rows, device=DEV)
+    c.rms_norm_forward(x, weight, rstd=rstd)
+    dx, dweight = torch.empty_like(x), torch.empty_like(weight)
+    c.rms_norm_backward(x, weight, rstd, dx, dweight, dy, accumulate=False)
+    want_x, want_w = norm_back64(x.double(), weight.double(), rstd.double(), dy.double())
+    n = (x.double() * rstd.double()[:, None]).abs()
+    u = (dy.double() * weight.double()).abs()
+    within(dx, want_x, stored(want_x, rstd.double()[:, None] * (u * 2.0 ** -21 + n * (u * n).mean(1, keepdim=True) * (cols * 2.0 ** -23 + 2.0 ** -20)), dtype), "dx")
+    within(dweight, want_w, stored(want_w, (dy.double().abs() * n).sum(0) * (rows * 2.0 ** -23 + 2.0 ** -20), dtype), "dweight")
+    assert c.status() == 0
     c.close()
 
 
