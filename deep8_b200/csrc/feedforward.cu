@@ -65,10 +65,10 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {  // read once: not
 // take every 16th k, each thread a pack of both projections, R products each in fp32.  The groups' sums meet in shared memory, the slices'
 // in scratch memory: the CTA that finishes a strip last adds them in slice order and forms h.  fp32, 4096 -> 2 x 16384: 82 us for one row
 // (6.5 TB/s), 88 for two to four, 146 for eight, whose multiply-adds no longer fit behind the loads; the tensor cores take 228 us.
-template <typename T, int R>
-__global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T* __restrict__ x, const T* __restrict__ w, T* __restrict__ h, int rows, int cols,
-                                                         int width, int k_per_slice, float* __restrict__ partial, unsigned* arrivals, GatedTail tail) {
-    constexpr int V = 16 / sizeof(T), STRIP = 16 * V;
+template <int R>
+__global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const float* __restrict__ x, const float* __restrict__ w, float* __restrict__ h, int rows,
+                                                                        int cols, int width, int k_per_slice, float* __restrict__ partial, unsigned* arrivals, GatedTail tail) {
+    constexpr int V = 4, STRIP = 16 * V;
     constexpr int CHUNK = R > 4 ? 256 : 512;  // k staged at a time
     __shared__ alignas(16) float xs[CHUNK][R];
     __shared__ float sums[8][2 * R * V][16];
@@ -82,11 +82,11 @@ __global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T*
         __syncthreads();
         for (int i = threadIdx.x; i < R * CHUNK; i += 256) {
             const int r = i / CHUNK, k = i % CHUNK;
-            xs[k][r] = r < rows && k < count ? widen(x[static_cast<size_t>(r) * cols + k0 + k]) : 0.0f;
+            xs[k][r] = r < rows && k < count ? x[static_cast<size_t>(r) * cols + k0 + k] : 0.0f;
         }
         __syncthreads();
         if (c < width) {
-            const T* wp = w + static_cast<size_t>(k0) * width + c;
+            const float* wp = w + static_cast<size_t>(k0) * width + c;
             constexpr int U = R > 4 ? 2 : 4;  // k per step: 2 U loads in flight
             for (int k0u = kl; k0u < count; k0u += 16 * U) {
                 uint4 gv[U], uv[U];
@@ -101,8 +101,8 @@ __global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T*
                 }
 #pragma unroll
                 for (int q = 0; q < U; ++q) {
-                    const T* ge = reinterpret_cast<const T*>(&gv[q]);
-                    const T* ue = reinterpret_cast<const T*>(&uv[q]);
+                    const float* ge = reinterpret_cast<const float*>(&gv[q]);
+                    const float* ue = reinterpret_cast<const float*>(&uv[q]);
                     // k is below CHUNK, a multiple of 16 U; from `count` on both factors are zeros
                     const Pack<float, R> a_row = *reinterpret_cast<const Pack<float, R>*>(xs[k0u + 16 * q]);
 #pragma unroll
@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T*
                         const float a = a_row.v[r];
 #pragma unroll
                         for (int j = 0; j < V; ++j) {
-                            g[r][j] = fmaf(a, widen(ge[j]), g[r][j]);
-                            u[r][j] = fmaf(a, widen(ue[j]), u[r][j]);
+                            g[r][j] = fmaf(a, ge[j], g[r][j]);
+                            u[r][j] = fmaf(a, ue[j], u[r][j]);
                         }
                     }
                 }
@@ -166,13 +166,13 @@ __global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T*
         }
         const size_t at = static_cast<size_t>(r) * width + col;
         if (tail.pre) {
-            static_cast<T*>(tail.pre)[at] = narrow<T>(gate);
-            static_cast<T*>(tail.pre)[tail.pre_stride + at] = narrow<T>(up);
+            static_cast<float*>(tail.pre)[at] = gate;
+            static_cast<float*>(tail.pre)[tail.pre_stride + at] = up;
         }
         float out = 0.0f;
         with_activation(tail.act, [&](auto which) {
             float value, slope;
-            activation<decltype(which)::value, sizeof(T) == 2, false>(gate, value, slope);
+            activation<decltype(which)::value, false, false>(gate, value, slope);
             out = value * up;
         });
         if (tail.dropping) {
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256, R > 2 ? 2 : 4) gated_rows_kernel(const T*
             const uint32_t word = (at & 3) == 0 ? words.x : (at & 3) == 1 ? words.y : (at & 3) == 2 ? words.z : words.w;
             out = drop_keeps(tail.drop, word) ? out * tail.drop.scale : 0.0f;
         }
-        h[at] = narrow<T>(out);
+        h[at] = out;
     }
 }
 
@@ -269,8 +269,11 @@ __global__ void __launch_bounds__(256) pad_kernel(PadJobs jobs, int count) {
     }
 }
 
-// dpre from pre and dz: five accesses per element, bound by HBM (8192 x 16384 fp16: 205 us, 6.5 TB/s; 250 behind a hot product).  pre and dpre may be the same
+// dpre from pre and dz: five accesses per element, bound by HBM (8192 x 16384 fp16: 211 us, 6.4 TB/s; 250 behind a hot product).  pre and dpre may be the same
 // memory (an element is read and written by one thread), so nothing here is declared __restrict__.
+// dpre is rounded to the tensors' type: the two products behind it take their operands in that type on the tensor cores, and an fp16 pair for
+// each value would double their 3.3 ms.  fp16 gradients are 3.0e-4 off in norm for it, 2.1e-4 without; values of dpre below 2^-14 lose bits and
+// below 2^-25 vanish, as everywhere between fp16 operators, which is what scaling the loss is for.
 template <int ACT, typename T, int E>
 __device__ __forceinline__ void gated_grad_elements(Pack<T, E>& g, Pack<T, E>& u, const Pack<T, E>& d, size_t i0, unsigned long long offset, const DropSpec& drop,
                                                     int dropping) {
@@ -464,8 +467,8 @@ __global__ void __launch_bounds__(512) rms_norm_forward_kernel(const T* x, const
 
 // dx (+)= and this CTA's part of dweight (partial[blockIdx.x][cols]) in one pass over x and dy: the columns a thread holds are the same for
 // every row, so their sums stay in its registers.  The next row's loads are issued before this row's sum is formed.
-// 8192 x 4096: fp16 40.7 us and 6.5 for the slices' sum (4.3 TB/s together), bound by instructions (23 per element) at 16 warps per SM; fp32
-// 63 + 3 us (6.1 TB/s).  Two packs per thread: 53 us with one, 65 with four.  Without the early loads fp32 took 82; a ring of rows in shared
+// 8192 x 4096: fp16 40.7 us and 6.5 for the slices' sum (4.3 TB/s together), bound by latency for want of warps: at 114 registers one CTA of 16
+// fits an SM, half of the issue slots and half of the memory's bandwidth go unused (23 instructions per element); fp32 63 + 3 us (6.1 TB/s).  Two packs per thread: 53 us with one, 65 with four.  Without the early loads fp32 took 82; a ring of rows in shared
 // memory filled by cp.async was no faster.
 template <typename T, int W, int N>
 __global__ void __launch_bounds__(512) rms_norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ weight, const float* __restrict__ rstd,
@@ -717,9 +720,9 @@ unsigned grid_for(const d8k_ctx* ctx, Kernel* kernel, size_t steps, int most_per
 }
 
 // The launch's form of a dropout argument; *on stays 0 when there is nothing to drop (none given, or p == 0).
-int make_drop(const d8k_dropout* drop, DropSpec* spec, int* on) {
+int make_drop(const d8k_dropout* drop, DropSpec* spec, int* on = nullptr) {
     *spec = DropSpec{0, 0, nullptr, 0, 1, 1.0f};
-    *on = 0;
+    if (on) *on = 0;
     if (!drop) return 0;
     if (!(drop->p >= 0.0 && drop->p <= 1.0)) return fail(D8K_ERR_ARGUMENT, "dropout: p must be between 0 and 1");
     if (reinterpret_cast<uintptr_t>(drop->device_offset) & 7) return fail(D8K_ERR_ARGUMENT, "dropout: device_offset must be 8-byte aligned");
@@ -730,7 +733,7 @@ int make_drop(const d8k_dropout* drop, DropSpec* spec, int* on) {
     spec->some = threshold < 4294967296.0;
     spec->threshold = spec->some ? static_cast<uint32_t>(threshold) : 0xffffffffu;
     spec->scale = spec->some ? static_cast<float>(1.0 / (1.0 - drop->p)) : 0.0f;
-    *on = drop->p > 0.0;
+    if (on) *on = drop->p > 0.0;
     return 0;
 }
 
@@ -749,7 +752,7 @@ bool gated_rows(d8k_ctx* ctx, const float* x, const float* w, float* h, int rows
     const int strips = (width + 16 * V - 1) / (16 * V);
     if (rows > 8 || width % V != 0 || !aligned16({w}) || strips > kMaxCounters) return false;
     const int r = rows <= 2 ? rows : rows <= 4 ? 4 : 8;
-    auto kernel = r == 1 ? gated_rows_kernel<float, 1> : r == 2 ? gated_rows_kernel<float, 2> : r == 4 ? gated_rows_kernel<float, 4> : gated_rows_kernel<float, 8>;
+    auto kernel = r == 1 ? gated_rows_kernel<1> : r == 2 ? gated_rows_kernel<2> : r == 4 ? gated_rows_kernel<4> : gated_rows_kernel<8>;
     long long slices = static_cast<long long>(ctx->num_sms) * resident_ctas(kernel, 256) / strips;
     if (slices > cols / 64) slices = cols / 64;
     const long long most = static_cast<long long>(ctx->scratch_bytes / (static_cast<size_t>(strips) * 2 * r * 16 * V * sizeof(float)));
@@ -898,8 +901,7 @@ int gated_grad_w(d8k_ctx* ctx, int dtype, void* dw, int rows, int xc, int yc, co
 int dropout(d8k_ctx* ctx, int dtype, const void* x, const void* residual, void* y, size_t n, const d8k_dropout* drop) {
     if (!drop) return fail(D8K_ERR_ARGUMENT, "dropout: null pointer");
     DropSpec spec;
-    int dropping = 0;
-    if (int rc = make_drop(drop, &spec, &dropping)) return rc;
+    if (int rc = make_drop(drop, &spec)) return rc;
     if (n == 0) return 0;
     if (!x || !y) return fail(D8K_ERR_ARGUMENT, "dropout: null pointer");
     const size_t bytes = n * esize(dtype);

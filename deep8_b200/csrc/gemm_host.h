@@ -39,7 +39,7 @@ struct HostOperand {
     long long ld2 = 0;
     long long batch_stride = 0;
     int batch_count = 1;
-    bool padded = false;       // a stored matrix whose rows go on as zeros to the next multiple of 128 bytes (pad_operands)
+    bool padded = false;       // a stored matrix whose rows go on as zeros to the next multiple of 128 bytes (launch_pad)
     ConvRule cr = {};
     // halo != 0 (set by run_gemm, fp32 only): the virtual matrix is fetched as per-tile patches of halo_rows x halo_wp pixels
     int halo = 0, halo_wp = 0, halo_rows = 0;

@@ -30,7 +30,7 @@
 //
 // GATED: B is a pair of matrices and a tile's columns are half of each, so that one accumulator row holds both projections of the same
 // outputs; the epilogue forms act(gate) * up, the dropout, and stores the projections too when the backward pass is to come.
-// PRECISE (fp32): chains of four k-blocks instead of sixteen per fp32 sum, the small terms in columns of their own.
+// PRECISE (fp32): chains of four k-blocks instead of eight per fp32 sum, the small terms in columns of their own.
 //
 // Every mbarrier wait is bounded: on expiry the CTA records a status code, all roles leave their loops, and the
 // kernel returns through the normal teardown (TMEM freed).

@@ -306,7 +306,8 @@ D8K_API int d8k_gated_grad_x_into(d8k_ctx* ctx, int dtype, void* dx, int xb, int
 D8K_API int d8k_gated_grad_w_into(d8k_ctx* ctx, int dtype, const void* x, int xb, int xr, int xc, void* dw, int yc, const void* dpre,
                                   int accumulate);
 /* The three above: dpre from pre and dz, then dx and dw; dx or dw may be NULL.  dpre (2 x rows x yc) is workspace, its contents afterwards
- * unspecified; it may be pre, which is then overwritten.
+ * unspecified; it may be pre, which is then overwritten.  Between the passes dpre is held in the tensors' type: D8K_F16 gradients are off by about
+ * 3e-4 in norm (2e-4 is their own rounding), and a dpre below 2^-25 counts as 0, so small losses want scaling as with any D8K_F16 gradient.
  * Rows that do not start on 16-byte boundaries (an odd xc or yc) are copied with padding before these products and d8k_gated_forward read
  * them: the first call of a size may allocate the copies' memory, which the context keeps; make it before any stream capture (inside
  * one, slower kernels that need no copies run instead when the memory is not there). */
