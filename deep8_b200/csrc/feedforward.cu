@@ -468,8 +468,9 @@ __global__ void __launch_bounds__(512) rms_norm_forward_kernel(const T* x, const
 // dx (+)= and this CTA's part of dweight (partial[blockIdx.x][cols]) in one pass over x and dy: the columns a thread holds are the same for
 // every row, so their sums stay in its registers.  The next row's loads are issued before this row's sum is formed.
 // 8192 x 4096: fp16 40.7 us and 6.5 for the slices' sum (4.3 TB/s together), bound by latency for want of warps: at 114 registers one CTA of 16
-// fits an SM, half of the issue slots and half of the memory's bandwidth go unused (23 instructions per element); fp32 63 + 3 us (6.1 TB/s).  Two packs per thread: 53 us with one, 65 with four.  Without the early loads fp32 took 82; a ring of rows in shared
-// memory filled by cp.async was no faster.
+// fits an SM, half of the issue slots and half of the memory's bandwidth go unused (23 instructions per element); fp32 63 + 3 us (6.1 TB/s).
+// Two packs per thread: 53 us with one, 65 with four.  Without the early loads fp32 took 82; a ring of rows in shared memory filled by cp.async
+// was no faster.
 template <typename T, int W, int N>
 __global__ void __launch_bounds__(512) rms_norm_backward_kernel(const T* __restrict__ x, const T* __restrict__ weight, const float* __restrict__ rstd,
                                                                 T* dx, float* __restrict__ partial, const T* __restrict__ dy, size_t rows, int cols,

@@ -39,8 +39,8 @@ __device__ __forceinline__ void sigmoid_and_rest(float a, float& s, float& c) {
 // value = act(a); slope = act'(a) when wanted.  gelu goes through erfc, gelu_tanh through a sigmoid ((1 + tanh z) / 2 = sigmoid(2 z)):
 // both forms keep the relative accuracy of the negative tail, where 1 + erf and 1 + tanh cancel.  FAST: the normal distribution's tail
 // beyond |a| is exp(-a^2 / 2) q(|a|), and q a polynomial of degree 7 in 1 / (1 + 0.264 |a|) without a constant, fitted for the least largest
-// relative error over |a| <= 14 (linear programming on 1200 Chebyshev points: 5.8e-7 as fitted, 8.9e-7 with these coefficients in 32 bits); the library's erfc made the fp16 product of
-// 1531 x 1024 by two of 1024 x 4096 a third longer than the other activations.  Factors beyond +-110 count as 110 where what they multiply has
+// relative error over |a| <= 14 (linear programming on 1200 Chebyshev points: 5.8e-7 as fitted, 8.9e-7 with these coefficients in 32 bits); the
+// library's erfc made the fp16 product of 1531 x 1024 by two of 1024 x 4096 a third longer than the other activations.  Factors beyond +-110 count as 110 where what they multiply has
 // vanished (exp(-104) is below the smallest float; an infinite projection times a vanished factor would be a NaN).
 template <int ACT, bool FAST, bool SLOPE>
 __device__ __forceinline__ void activation(float a, float& value, float& slope) {
